@@ -54,6 +54,19 @@ class MelPlan(C.Structure):
                 ("fb_count", C.c_void_p), ("fb_w", C.c_void_p)]
 
 
+class Pages(C.Structure):
+    _fields_ = ([("k", C.c_void_p), ("v", C.c_void_p)]
+                + [(n, C.c_longlong) for n in ("k_page", "k_head", "k_slot", "v_page", "v_head", "v_slot")]
+                + [(n, C.c_int) for n in ("n_pages", "page_size", "kv_heads", "head_dim")])
+
+
+class PageRows(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "block_table", "kv_lens", "cu_rows")]
+                + [(n, C.c_longlong) for n in ("q_row", "q_head", "table_row")]
+                + [(n, C.c_int) for n in ("batch", "rows", "heads", "table_width", "window", "sinks", "causal", "max_rows")]
+                + [("scale", C.c_float)])
+
+
 class StreamLanes(C.Structure):
     _fields_ = [("n", C.c_int), ("streams", C.c_void_p * 7), ("events", C.c_void_p * 8)]
 
@@ -113,6 +126,11 @@ _SIGNATURES = {
                                             _vp, C.POINTER(StreamLanes)]),
     "fcenc_greedy_decode": (C.c_int, [_fp, _i, _fp, _fp, _fp, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _vp, _vp, _vp]),
     "fcenc_mel_spectrogram": (C.c_int, [C.POINTER(MelPlan), _fp, C.c_longlong, _vp, _i, _i, _fp, _i, _vp, _vp]),
+    "fcenc_page_plan": (C.c_int, [_vp, _vp, _vp, _i, _vp, C.c_longlong, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp]),
+    "fcenc_page_write": (C.c_int, [_i, C.POINTER(Pages), _vp, _vp] + [C.c_longlong] * 4 + [_vp, _i, _vp]),
+    "fcenc_page_attention_workspace_bytes": (C.c_size_t, [_i, C.POINTER(Pages), C.POINTER(PageRows)]),
+    "fcenc_page_attention": (C.c_int, [_i, C.POINTER(Pages), C.POINTER(PageRows), _vp, _vp, C.c_size_t, _vp]),
+    "fcenc_sample_tokens": (C.c_int, [_i, _vp, C.c_longlong, _i, _i, _fp, _fp, _vp, _fp, _fp, _vp, _vp]),
     "fcenc_out_frames": (C.c_int, [_i]),
     "fcenc_padded_frames": (C.c_int, [_i]),
     "fcenc_event_create": (C.c_void_p, []),

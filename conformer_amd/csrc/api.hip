@@ -821,6 +821,73 @@ int fcenc_greedy_decode(const float* enc_proj, int ldj, const float* pred_proj, 
   return launch_greedy_decode(a, (hipStream_t)stream);
 }
 
+int fcenc_page_plan(int32_t* kv_lens, const int32_t* new_lens, const uint8_t* finished, int B, int32_t* block_table,
+                    long long table_row, int table_width, int32_t* free_pages, int32_t* free_count, int pool_pages,
+                    int page_size, int64_t* slots, int rows, int32_t* cu_rows, uint8_t* granted, void* stream) {
+  PagePlanArgs a;
+  a.kv_lens = kv_lens; a.new_lens = new_lens; a.finished = finished; a.B = B; a.table = block_table; a.table_row = table_row;
+  a.width = table_width; a.free_pages = free_pages; a.free_count = free_count; a.pool = pool_pages;
+  a.shift = page_shift(page_size); a.slots = slots; a.rows = rows; a.cu_rows = cu_rows; a.granted = granted;
+  return launch_page_plan(a, (hipStream_t)stream);
+}
+
+static int element_bytes(int dtype) { return dtype == FCENC_BF16 ? 2 : dtype == FCENC_F32 ? 4 : 0; }
+
+int fcenc_page_write(int dtype, const fcenc_pages* pages, const void* k, const void* v, long long k_row, long long k_head,
+                     long long v_row, long long v_head, const int64_t* slots, int rows, void* stream) {
+  const int es = element_bytes(dtype);
+  if (!es) return fail("page_write: dtype %d", dtype);
+  if (!pages) return fail("page_write: null pages");
+  PageWriteArgs a;
+  a.k = (const char*)k; a.v = (const char*)v; a.k_pages = (char*)pages->k; a.v_pages = (char*)pages->v; a.slots = slots;
+  a.k_row = k_row * es; a.k_head = k_head * es; a.v_row = v_row * es; a.v_head = v_head * es;
+  a.k_page = pages->k_page * es; a.k_phead = pages->k_head * es; a.k_slot = pages->k_slot * es;
+  a.v_page = pages->v_page * es; a.v_phead = pages->v_head * es; a.v_slot = pages->v_slot * es;
+  a.rows = rows; a.heads = pages->kv_heads; a.head_bytes = pages->head_dim * es; a.n_pages = pages->n_pages;
+  a.shift = page_shift(pages->page_size);
+  return launch_page_write(a, (hipStream_t)stream);
+}
+
+static int page_attn_args(int dtype, const fcenc_pages* p, const fcenc_page_rows* r, PageAttnArgs& a) {
+  const int es = element_bytes(dtype);
+  if (!es) return fail("page_attention: dtype %d", dtype);
+  if (!p || !r) return fail("page_attention: null descriptor");
+  const long long slot_max = 1ll << 30;
+  if (p->k_slot < 0 || p->v_slot < 0 || p->k_slot * es > slot_max || p->v_slot * es > slot_max) return fail("page_attention: slot strides %lld / %lld", p->k_slot, p->v_slot);
+  a.q = (const char*)r->q; a.k = (const char*)p->k; a.v = (const char*)p->v;
+  a.table = r->block_table; a.kv_lens = r->kv_lens; a.cu_rows = r->cu_rows;
+  a.q_row = r->q_row * es; a.q_head = r->q_head * es;
+  a.k_page = p->k_page * es; a.k_head = p->k_head * es; a.k_slot = (int)(p->k_slot * es);
+  a.v_page = p->v_page * es; a.v_head = p->v_head * es; a.v_slot = (int)(p->v_slot * es);
+  a.table_row = r->table_row; a.width = r->table_width; a.B = r->batch; a.rows = r->rows; a.heads = r->heads;
+  a.kv_heads = p->kv_heads; a.dim = p->head_dim; a.n_pages = p->n_pages; a.shift = page_shift(p->page_size);
+  a.window = r->window; a.sinks = r->sinks; a.causal = r->causal; a.max_rows = r->max_rows; a.scale = r->scale;
+  return 0;
+}
+
+size_t fcenc_page_attention_workspace_bytes(int dtype, const fcenc_pages* pages, const fcenc_page_rows* rows) {
+  PageAttnArgs a;
+  if (page_attn_args(dtype, pages, rows, a)) return 0;
+  return page_attention_workspace_bytes(dtype, a);
+}
+
+int fcenc_page_attention(int dtype, const fcenc_pages* pages, const fcenc_page_rows* rows, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  PageAttnArgs a;
+  if (page_attn_args(dtype, pages, rows, a)) return -1;
+  a.out = (char*)out; a.ws = (float*)workspace;
+  return launch_page_attention(dtype, a, workspace_bytes, (hipStream_t)stream);
+}
+
+int fcenc_sample_tokens(int dtype, const void* logits, long long row_stride, int rows, int vocab, const float* u,
+                        const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                        int32_t* tokens, void* stream) {
+  SampleArgs a;
+  a.logits = logits; a.row_stride = row_stride; a.rows = rows; a.vocab = vocab; a.u = u; a.temperature = temperature;
+  a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.tokens = tokens;
+  return launch_sample_tokens(dtype, a, (hipStream_t)stream);
+}
+
 int fcenc_mel_spectrogram(const fcenc_mel_plan* plan, const float* wave, long long ldw, const int64_t* lengths, int B,
                           int S, float* mel, int Tmax, int64_t* frames, void* stream) {
   if (!plan) return fail("mel: null plan");

@@ -286,6 +286,60 @@ struct MelArgs {
 };
 int launch_mel_spectrogram(const MelArgs& a, hipStream_t stream);
 
+// pages of a key/value cache (see pages.hip); `shift` = log2 of the page size, -1 for a size that is not allowed
+int page_shift(int page_size);
+struct PagePlanArgs {
+  int32_t* kv_lens = nullptr;         // [B] tokens every row holds, advanced by the plan
+  const int32_t* new_lens = nullptr;  // [B] rows every request brings
+  const uint8_t* finished = nullptr;  // [B] or null: rows to empty first
+  int32_t* table = nullptr;           // [B][table_row] page ids
+  int32_t* free_pages = nullptr;      // [pool] stack of pages that nobody holds
+  int32_t* free_count = nullptr;      // its height
+  int64_t* slots = nullptr;           // [rows]
+  int32_t* cu_rows = nullptr;         // [B + 1]
+  uint8_t* granted = nullptr;         // [B]
+  long long table_row = 0;
+  int B = 0, width = 0, pool = 0, rows = 0, shift = 0;
+};
+int launch_page_plan(const PagePlanArgs& a, hipStream_t stream);
+// strides in bytes
+struct PageWriteArgs {
+  const char *k = nullptr, *v = nullptr;
+  char *k_pages = nullptr, *v_pages = nullptr;
+  const int64_t* slots = nullptr;
+  long long k_row = 0, k_head = 0, v_row = 0, v_head = 0;
+  long long k_page = 0, k_phead = 0, k_slot = 0, v_page = 0, v_phead = 0, v_slot = 0;
+  int rows = 0, heads = 0, head_bytes = 0, n_pages = 0, shift = 0;
+};
+int launch_page_write(const PageWriteArgs& a, hipStream_t stream);
+// attention of a chunk of new rows over the pages (see page_attn.hip); strides in bytes
+struct PageAttnArgs {
+  const char *q = nullptr, *k = nullptr, *v = nullptr;
+  const int32_t *table = nullptr, *kv_lens = nullptr, *cu_rows = nullptr;
+  char* out = nullptr;                // [rows][heads][dim]
+  float* ws = nullptr;                // partial results of a split key axis
+  long long q_row = 0, q_head = 0, k_page = 0, k_head = 0, v_page = 0, v_head = 0, table_row = 0;
+  int k_slot = 0, v_slot = 0;
+  int B = 0, rows = 0, heads = 0, kv_heads = 0, dim = 0, n_pages = 0, width = 0, shift = 0;
+  int window = 0, sinks = 0, causal = 1, max_rows = 0;
+  float scale = 1.f;
+};
+size_t page_attention_workspace_bytes(int dtype, const PageAttnArgs& a);
+int launch_page_attention(int dtype, const PageAttnArgs& a, size_t ws_bytes, hipStream_t stream);
+// token sampling (see sample.hip)
+struct SampleArgs {
+  const void* logits = nullptr;       // [rows][row_stride]
+  const float* u = nullptr;           // [rows] in [0, 1)
+  const float* temperature = nullptr; // [rows] or null (1)
+  const int32_t* top_k = nullptr;     // [rows] or null (off)
+  const float* top_p = nullptr;       // [rows] or null (off)
+  const float* min_p = nullptr;       // [rows] or null (off)
+  int32_t* tokens = nullptr;          // [rows]
+  long long row_stride = 0;           // elements
+  int rows = 0, vocab = 0;
+};
+int launch_sample_tokens(int dtype, const SampleArgs& a, hipStream_t stream);
+
 int stream_max_chunk_frames();    // largest Tq the two kernels above take
 int stream_max_cache_frames();    // largest cap
 

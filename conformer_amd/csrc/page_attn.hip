@@ -1,0 +1,456 @@
+// Attention of a chunk of new rows over a paged key/value cache (gfx950).
+//
+// Request b brings rows cu_rows[b] .. cu_rows[b + 1] - 1 (n of them) and holds kv = kv_lens[b] tokens, the chunk's own
+// among them: its row i sits at position p = kv - n + i and sees the tokens j with
+//     j < kv,   causal: j <= p,   window w > 0: j > p - w or j < sinks.
+//   out = softmax_j(scale * q . k_j) . v_j;   a row that sees nothing gives zeros.
+// Query head h reads kv head h / (heads / kv_heads).  Token j is slot j mod page_size of page table[b][j / page_size]; the
+// tokens of a page whose id is outside the pool are seen by nobody.
+//
+// One pass over the keys with a running maximum m and sum l per row (fp32, base-2 exponents):
+//     m' = max(m, max_j s_j),  l' = l 2^(m - m') + sum_j 2^(s_j - m'),  O' = O 2^(m - m') + sum_j 2^(s_j - m') v_j.
+//
+// A tile is a set of rows of one (request, kv head): `tt` neighbouring rows of the chunk times the gc query heads that
+// share the kv head, so that a key read once serves all of them.  Workgroup t finds its request without any table:
+// start(b) = cu_rows[b] / tt + b grows by at least ceil(n / tt) from one request to the next, so the request of t is
+// the last one with start(b) <= t, and rows / tt + B + 1 workgroups cover every batch.
+//
+// Everything is computed transposed: S^T = K Q^T has the query row on the lane's column and tokens on the accumulator
+// rows, and those rows are, as they are, the k elements of the B operand of O^T = V^T P^T once the V fragment is read
+// in the same token order.  P never leaves the registers; V^T fragments come out of LDS with transposing reads.
+//
+// Loads of K and V go through a buffer descriptor per 16 tokens of a page (pages hold at least 16) whose size ends behind the
+// last token that the tile sees: what lies beyond (stale slots, head dims up to the padded width, bad pages) loads
+// as zero, so garbage there can reach neither the scores nor, as 0 * NaN, the sums.
+#include <math.h>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace fcenc {
+
+namespace {
+
+constexpr uint32_t OOB = 0xF0000000u;       // an offset outside every descriptor
+constexpr int MAX_SPLITS = 64;
+constexpr int STEP_WAVES = 4;
+constexpr int STEP_ROWS = 16;
+
+struct TileInfo {
+  int b, t0, n, c0, kv;                      // request (B: rows behind the last one), first row, rows, offset, tokens
+};
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int clamp_rows(int v, int rows) { return v < 0 ? 0 : (v > rows ? rows : v); }
+
+// false: no such tile
+__device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, int tt, TileInfo& ti) {
+  int lo = 0, hi = a.B + 1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int start = clamp_rows(uniform(a.cu_rows[mid]), a.rows) / tt + mid;
+    if (start <= tile) lo = mid; else hi = mid;
+  }
+  ti.b = lo;
+  ti.c0 = clamp_rows(uniform(a.cu_rows[lo]), a.rows);
+  const int c1 = lo < a.B ? clamp_rows(uniform(a.cu_rows[lo + 1]), a.rows) : a.rows;
+  ti.n = c1 - ti.c0;
+  ti.t0 = (tile - (ti.c0 / tt + lo)) * tt;
+  ti.kv = 0;
+  if (ti.t0 < 0 || ti.t0 >= ti.n) return false;
+  if (lo < a.B) {
+    const int cap = a.width << a.shift, kv = uniform(a.kv_lens[lo]);
+    ti.kv = kv < 0 ? 0 : (kv > cap ? cap : kv);
+  }
+  return true;
+}
+
+// V^T fragment of a [32 tokens][DP] tile in LDS: element j of lane (g, r) is V[token 16 (j >> 2) + 4 g + (j & 3)][dim 16 db + r]
+template <int ROWB>
+__device__ __forceinline__ bf16x8 v_frag(const char* vt, int db, int g, int r, bf16) {
+  using lds_bf16x4 = __attribute__((address_space(3))) bf16x4;
+  bf16x8 f;
+#pragma unroll
+  for (int hi = 0; hi < 2; ++hi) {
+    const int key = 16 * hi + 4 * g + (r >> 2);
+    const char* p = vt + tile_off<ROWB>(key, 2 * db + ((r & 3) >> 1)) + 8 * (r & 1);
+    const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f[4 * hi + q] = v[q];
+  }
+  return f;
+}
+template <int ROWB>
+__device__ __forceinline__ f32x8 v_frag(const char* vt, int db, int g, int r, float) {
+  f32x8 f;
+  const int dv = 16 * db + r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int key = 16 * (j >> 2) + 4 * g + (j & 3);
+    const float v = *reinterpret_cast<const float*>(vt + tile_off<ROWB>(key, dv >> 2) + 4 * (dv & 3));
+    if (j < 4) f.lo[j] = v; else f.hi[j - 4] = v;
+  }
+  return f;
+}
+__device__ __forceinline__ bf16x8 p_frag(const float (&x)[8], bf16) {
+  bf16x8 f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (bf16)x[i];
+  return f;
+}
+__device__ __forceinline__ f32x8 p_frag(const float (&x)[8], float) {
+  f32x8 f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f.lo[i] = x[i];
+    f.hi[i] = x[4 + i];
+  }
+  return f;
+}
+
+// eight elements of a row through a descriptor
+__device__ __forceinline__ bf16x8 load_frag(__amdgpu_buffer_rsrc_t r, uint32_t off, bf16) {
+  return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+__device__ __forceinline__ f32x8 load_frag(__amdgpu_buffer_rsrc_t r, uint32_t off, float) {
+  f32x8 f;
+  f.lo = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+  f.hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 16, 0));
+  return f;
+}
+
+__device__ __forceinline__ void store_row(bf16* p, float v) { *p = (bf16)v; }
+__device__ __forceinline__ void store_row(float* p, float v) { *p = v; }
+
+// ---------------------------------------------------------------------------------------------------------------
+// Tiles of up to 16 rows: single tokens and short chunks.  Bound by the bytes of K and V.  The four waves of a workgroup
+// take every fourth block of 32 tokens, on their own (K straight into MFMA fragments, V through a wave-private LDS
+// tile), with the next block's loads in flight; their partial results meet in LDS.  With few tiles the key axis is
+// also cut into `splits` pieces, whose results a second launch joins.
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int DP>
+struct StepTile {
+  static constexpr int ROWB = DP * (int)sizeof(T);
+  static constexpr int CPR = ROWB / 16;                     // 16-byte pieces of a row
+  static constexpr int OROW = DP + 4;                       // floats per row of the merge buffer
+  static constexpr int WAVE_BYTES = 32 * ROWB > STEP_ROWS * OROW * 4 ? 32 * ROWB : STEP_ROWS * OROW * 4;
+  static constexpr int BYTES = STEP_WAVES * WAVE_BYTES + STEP_WAVES * STEP_ROWS * 8;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 ? 1 : 2))
+    page_attn_step_kernel(const PageAttnArgs a, int gc, int hchunks, int tt, int splits) {
+  using TL = StepTile<T, DP>;
+  using Frag = typename Traits<T>::Frag;
+  constexpr int ROWB = TL::ROWB, CPR = TL::CPR, ES = (int)sizeof(T);
+  constexpr int KS = DP / 32, NDB = DP / 16, NV = CPR / 4;   // k32 steps, 16-dim blocks, V loads per 16 tokens
+  constexpr int RPI = 64 / CPR;                              // V rows per load instruction
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  const int kvh = blockIdx.y / hchunks, hc = blockIdx.y - kvh * hchunks;
+  const int split = blockIdx.z;
+  const int group = a.heads / a.kv_heads;
+
+  TileInfo ti;
+  if (!find_tile(a, blockIdx.x, tt, ti)) return;
+  const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
+  const int last = first + (ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt) - 1;
+  int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
+  if (ti.b == a.B || hi < 0) hi = 0;
+  int lo = a.window > 0 ? first - a.window + 1 : 0;
+  lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
+  const int sinks = a.window > 0 ? a.sinks : 0;
+  const int lob = lo >> 5;
+  int sb = ((sinks < hi ? sinks : hi) + 31) >> 5;
+  sb = sb < lob ? sb : lob;
+  const int count = hi > 0 ? sb + ((hi + 31) >> 5) - lob : 0;
+  const int i0 = (int)((long long)count * split / splits), i1 = (int)((long long)count * (split + 1) / splits);
+
+  // this lane's row of the tile
+  const int rt = r / gc, rh = hc * gc + r - rt * gc;
+  const bool live = rt < tt && ti.t0 + rt < ti.n && rh < group;
+  const int pos = first + rt;
+  const int see_hi = a.causal ? pos : ti.kv - 1;             // last token it sees
+  const int see_lo = a.window > 0 ? pos - a.window + 1 : 0;  // first one, next to the sinks
+  Frag q[KS];
+  {
+    const char* qrow = a.q + (long long)(ti.c0 + ti.t0 + (live ? rt : 0)) * a.q_row + (long long)(kvh * group + (live ? rh : 0)) * a.q_head;
+    const __amdgpu_buffer_rsrc_t none = buffer_of(nullptr, 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      q[ks] = load_frag(none, OOB, T{});
+      if (live && 32 * ks + 8 * g < a.dim) q[ks] = *reinterpret_cast<const Frag*>(qrow + (32 * ks + 8 * g) * ES);
+    }
+  }
+
+  f32x4 ot[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i) ot[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.f;
+  const float c = a.scale * kLog2e;
+  char* vt = smem + wave * TL::WAVE_BYTES;
+  const int32_t* trow = a.table + (long long)(ti.b < a.B ? ti.b : 0) * a.table_row;
+  const char* kbase = a.k + kvh * a.k_head;
+  const char* vbase = a.v + kvh * a.v_head;
+
+  Frag kf[2][KS];
+  u32x4 vr[2][NV];
+  bool page_ok[2];
+  auto block_of = [&](int i) { return i < sb ? i : lob + i - sb; };
+  // descriptors of the 16 tokens from tok0 on: bytes up to the last one that the tile sees
+  auto fetch = [&](int i) {
+    const int j0 = block_of(i) * 32;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int tok0 = j0 + 16 * t;
+      int left = hi - tok0;
+      left = left > 16 ? 16 : left;
+      int page = -1;
+      if (left > 0) page = uniform(trow[tok0 >> a.shift]);
+      const bool ok = page >= 0 && page < a.n_pages;
+      page_ok[t] = ok || left <= 0;
+      const int slot0 = tok0 & ((1 << a.shift) - 1);
+      const char* kp = kbase + (long long)(ok ? page : 0) * a.k_page + (long long)slot0 * a.k_slot;
+      const char* vp = vbase + (long long)(ok ? page : 0) * a.v_page + (long long)slot0 * a.v_slot;
+      const __amdgpu_buffer_rsrc_t kd = buffer_of(kp, ok ? (left - 1) * a.k_slot + a.dim * ES : 0);
+      const __amdgpu_buffer_rsrc_t vd = buffer_of(vp, ok ? (left - 1) * a.v_slot + a.dim * ES : 0);
+      // tokens in front of the window and behind the sinks are seen by no row of the tile
+      const bool dead_k = tok0 + r < lo && tok0 + r >= sinks;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int d0 = 32 * ks + 8 * g;
+        kf[t][ks] = load_frag(kd, dead_k || d0 >= a.dim ? OOB : (uint32_t)(r * a.k_slot + d0 * ES), T{});
+      }
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int row = lane / CPR + v * RPI, ch = lane % CPR;
+        const bool dead_v = tok0 + row < lo && tok0 + row >= sinks;
+        vr[t][v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(dead_v || ch * 16 >= a.dim * ES ? OOB : (uint32_t)(row * a.v_slot + ch * 16)), 0, 0);
+      }
+    }
+  };
+
+  int i = i0 + wave;
+  if (i < i1) fetch(i);
+  for (; i < i1; i += STEP_WAVES) {
+    const int j0 = block_of(i) * 32;
+    const bool ok0 = page_ok[0], ok1 = page_ok[1];
+    // ---- S^T = K Q^T: lane (g, r), register e of tile t: token j0 + 16 t + 4 g + e, row r ----
+    f32x4 st[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) mma(st[t], kf[t][ks], q[ks]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");         // the tile of the block before has been read
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        *reinterpret_cast<u32x4*>(vt + tile_off<ROWB>(16 * t + lane / CPR + v * RPI, lane % CPR)) = vr[t][v];
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    if (i + STEP_WAVES < i1) fetch(i + STEP_WAVES);
+
+    bool inside = ok0 && ok1 && j0 + 31 <= (a.causal ? first : ti.kv - 1);
+    if (a.window > 0) inside = inside && (j0 >= last - a.window + 1 || j0 + 31 < sinks);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float s = st[t][e] * c;
+        if (!inside) {
+          const int j = j0 + 16 * t + 4 * g + e;
+          const bool see = (t ? ok1 : ok0) && j <= see_hi && (j >= see_lo || j < sinks);
+          s = see ? s : -INFINITY;
+        }
+        st[t][e] = s;
+      }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tmax = fmaxf(tmax, st[t][e]);
+    const float m_new = fmaxf(m_run, rows4_max(tmax));
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+    m_run = m_new;
+    float pk[8], psum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      pk[e] = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - m_use);
+      psum += pk[e];
+    }
+    l_run = l_run * alpha + psum;
+    // the probabilities are rounded to the storage type for the product; their sum is not
+    const Frag pf = p_frag(pk, T{});
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      ot[db] *= alpha;
+      mma(ot[db], v_frag<ROWB>(vt, db, g, r, T{}), pf);
+    }
+  }
+
+  // ---- the four waves' results ----
+  l_run = rows4_sum(l_run);
+  float* ob = reinterpret_cast<float*>(vt);
+  float2* ml = reinterpret_cast<float2*>(smem + STEP_WAVES * TL::WAVE_BYTES);
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) *reinterpret_cast<f32x4*>(ob + r * TL::OROW + 16 * db + 4 * g) = ot[db];
+  if (g == 0) ml[wave * STEP_ROWS + r] = float2{m_run, l_run};
+  __syncthreads();
+  constexpr int DPT = DP / 16;                              // dims per thread: 16 threads a row
+  const int row = tid >> 4, d0 = (tid & 15) * DPT;
+  const int ort = row / gc, orh = hc * gc + row - ort * gc;
+  if (!(ort < tt && ti.t0 + ort < ti.n && orh < group)) return;
+  float m = -INFINITY, l = 0.f, acc[DPT];
+#pragma unroll
+  for (int w = 0; w < STEP_WAVES; ++w) m = fmaxf(m, ml[w * STEP_ROWS + row].x);
+#pragma unroll
+  for (int d = 0; d < DPT; ++d) acc[d] = 0.f;
+#pragma unroll
+  for (int w = 0; w < STEP_WAVES; ++w) {
+    const float2 p = ml[w * STEP_ROWS + row];
+    if (p.y == 0.f) continue;                                // nothing seen by that wave
+    const float f = __builtin_amdgcn_exp2f(p.x - m);
+    l += p.y * f;
+    const float* src = reinterpret_cast<const float*>(smem + w * TL::WAVE_BYTES) + row * TL::OROW + d0;
+#pragma unroll
+    for (int d = 0; d < DPT; ++d) acc[d] += src[d] * f;
+  }
+  const long long orow = (long long)(ti.c0 + ti.t0 + ort) * a.heads + kvh * group + orh;
+  if (splits == 1) {
+    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);       // NaN stays NaN
+    T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
+#pragma unroll
+    for (int d = 0; d < DPT; ++d)
+      if (d0 + d < a.dim) store_row(o + d0 + d, acc[d] * inv);
+  } else {
+    const long long rows = (long long)a.rows * a.heads;
+    float* o = a.ws + 2 * rows * splits + (orow * splits + split) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DPT; ++d)
+      if (d0 + d < a.dim) o[d0 + d] = acc[d];
+    if ((tid & 15) == 0) reinterpret_cast<float2*>(a.ws)[orow * splits + split] = float2{m, l};
+  }
+}
+
+// joins the pieces of a split key axis: one wave per (row, head)
+template <typename T>
+__global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs a, int splits) {
+  const long long rows = (long long)a.rows * a.heads;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  float2 p{-INFINITY, 0.f};
+  if (lane < splits) p = reinterpret_cast<const float2*>(a.ws)[row * splits + lane];
+  float m = p.x;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float f = p.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.x - m);
+  float l = p.y * f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  const float* src = a.ws + 2 * rows * splits + row * splits * a.dim;
+  float acc[2] = {0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float w = __shfl(f, s);
+    if (w == 0.f) continue;                                  // a piece that saw nothing
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (lane + 64 * k < a.dim) acc[k] += w * src[(long long)s * a.dim + lane + 64 * k];
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (lane + 64 * k < a.dim) store_row(reinterpret_cast<T*>(a.out) + row * a.dim + lane + 64 * k, acc[k] * inv);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------------
+struct StepPlan {
+  int gc, hchunks, tt, tiles, splits;
+};
+
+StepPlan step_plan(const PageAttnArgs& a) {
+  StepPlan s;
+  const int group = a.heads / a.kv_heads;
+  s.gc = group < STEP_ROWS ? group : STEP_ROWS;
+  s.hchunks = (group + s.gc - 1) / s.gc;
+  s.tt = STEP_ROWS / s.gc;
+  s.tiles = a.rows / s.tt + a.B + 1;
+  // workgroups that have work, and how many pieces of the key axis fill the chip with four per CU; a piece is at
+  // least 256 tokens long for the longest request that the table can describe
+  const long long full = (a.rows + s.tt - 1) / s.tt, some = a.rows < a.B ? a.rows : a.B;
+  const long long busy = (full > some ? full : some) * a.kv_heads * s.hchunks;
+  long long longest = (long long)a.width << a.shift;
+  if (a.window > 0 && (long long)a.window + a.sinks + s.tt + 64 < longest) longest = (long long)a.window + a.sinks + s.tt + 64;
+  long long sp = busy > 0 ? 1024 / busy : 1;
+  if (sp > longest / 256) sp = longest / 256;
+  if (sp > MAX_SPLITS) sp = MAX_SPLITS;
+  s.splits = sp < 1 ? 1 : (int)sp;
+  return s;
+}
+
+size_t split_bytes(const PageAttnArgs& a, int splits) {
+  return splits > 1 ? (size_t)a.rows * a.heads * splits * (a.dim + 2) * sizeof(float) : 0;
+}
+
+int check_args(int dtype, const PageAttnArgs& a) {
+  const int es = dtype == DT_BF16 ? 2 : 4;
+  if (dtype != DT_BF16 && dtype != DT_F32) return fail("page_attention: dtype %d", dtype);
+  if (a.B <= 0 || a.rows < 0 || a.kv_heads <= 0 || a.heads <= 0 || a.heads % a.kv_heads) return fail("page_attention: B=%d rows=%d, %d heads over %d kv heads", a.B, a.rows, a.heads, a.kv_heads);
+  if (a.dim <= 0 || a.dim > 128 || a.dim % 8) return fail("page_attention: head dim %d unsupported (<= 128, multiple of 8)", a.dim);
+  if (a.shift < 0) return fail("page_attention: the page size must be a power of two, 16 to 1024");
+  if (a.n_pages <= 0 || a.width <= 0 || a.table_row < a.width) return fail("page_attention: %d pages, table of %d columns in rows of %lld", a.n_pages, a.width, a.table_row);
+  if (((long long)a.width << a.shift) > 0x7fffffffll - 64) return fail("page_attention: a table of %d pages describes too many tokens", a.width);
+  if (a.window < 0 || a.sinks < 0 || a.max_rows < 0) return fail("page_attention: window, sinks and max_rows must not be negative");
+  if (!(a.scale > 0.f) || !isfinite(a.scale)) return fail("page_attention: the scale must be positive and finite");
+  const long long strides[] = {a.q_row, a.q_head, a.k_page, a.k_head, a.k_slot, a.v_page, a.v_head, a.v_slot};
+  for (long long s : strides)
+    if (s % 16) return fail("page_attention: strides must be multiples of 16 bytes");
+  if (a.k_slot < a.dim * es || a.v_slot < a.dim * es || a.k_slot > (1 << 26) || a.v_slot > (1 << 26)) return fail("page_attention: slots of %d / %d bytes for %d dims", a.k_slot, a.v_slot, a.dim);
+  if ((long long)a.rows * a.heads > 0x7fffffffll || a.kv_heads > 65535) return fail("page_attention: too many rows or heads");
+  return 0;
+}
+
+template <typename T, int DP>
+int run_step(const PageAttnArgs& a, const StepPlan& s, hipStream_t stream) {
+  using TL = StepTile<T, DP>;
+  auto k = page_attn_step_kernel<T, DP>;
+  if (reserve_lds(reinterpret_cast<const void*>(k), TL::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", TL::BYTES);
+  k<<<dim3(s.tiles, a.kv_heads * s.hchunks, s.splits), 64 * STEP_WAVES, TL::BYTES, stream>>>(a, s.gc, s.hchunks, s.tt, s.splits);
+  if (s.splits > 1) {
+    const long long rows = (long long)a.rows * a.heads;
+    page_attn_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(a, s.splits);
+  }
+  return check_launch("page_attention");
+}
+
+}  // namespace
+
+size_t page_attention_workspace_bytes(int dtype, const PageAttnArgs& a) {
+  if (check_args(dtype, a) != 0) return 0;
+  return split_bytes(a, step_plan(a).splits);
+}
+
+int launch_page_attention(int dtype, const PageAttnArgs& a, size_t ws_bytes, hipStream_t stream) {
+  if (check_args(dtype, a) != 0) return -1;
+  if (a.rows == 0) return 0;
+  if (!a.q || !a.k || !a.v || !a.table || !a.kv_lens || !a.cu_rows || !a.out) return fail("page_attention: null operand");
+  if ((uintptr_t)a.q % 16 || (uintptr_t)a.k % 16 || (uintptr_t)a.v % 16) return fail("page_attention: operands must be 16-byte aligned");
+  const StepPlan s = step_plan(a);
+  const size_t need = split_bytes(a, s.splits);
+  if (need > 0 && (!a.ws || ws_bytes < need || (uintptr_t)a.ws % 16)) return fail("page_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  if (dtype == DT_BF16) return a.dim <= 64 ? run_step<bf16, 64>(a, s, stream) : run_step<bf16, 128>(a, s, stream);
+  return a.dim <= 64 ? run_step<float, 64>(a, s, stream) : run_step<float, 128>(a, s, stream);
+}
+
+}  // namespace fcenc

@@ -615,3 +615,175 @@ def _(enc_proj, pred_proj, out_w, out_b, d_joint, blank, max_symbols, clamp, cap
     return (torch.empty((b, capacity), dtype=torch.int32, device=enc_proj.device),
             torch.empty((b,), dtype=torch.int32, device=enc_proj.device),
             torch.empty((b,), dtype=torch.int32, device=enc_proj.device))
+
+
+# ------------------------------------------------------------------------------------------
+# pages of a key/value cache, attention over them, token sampling
+# ------------------------------------------------------------------------------------------
+def _on(t: Tensor, device: torch.device, dtype: torch.dtype, name: str, ndim: int) -> Tensor:
+    """An operand of the serving operators: on `device`, unit stride along its last dimension."""
+    if t.device != device or not t.is_cuda:
+        raise RuntimeError(f"fcenc: {name} must live on the GPU, beside the other operands (got {t.device}, {device})")
+    if t.dtype != dtype:
+        raise TypeError(f"fcenc: {name} must be {dtype}, got {t.dtype}")
+    if t.dim() != ndim:
+        raise ValueError(f"fcenc: {name} must have {ndim} dims, got {tuple(t.shape)}")
+    if t.numel() > 1 and t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"fcenc: {name} must be contiguous along its last dimension")
+    return t
+
+
+def _launch(device: torch.device, call, *args) -> None:
+    """`call` with `device` current: a kernel is launched on the device that is, whatever its stream belongs to."""
+    if device.index == torch.cuda.current_device():
+        rc = call(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = call(*args)
+    if rc != 0:
+        N.check(rc)
+
+
+def _pages(k_pages: Tensor, v_pages: Tensor, dev: torch.device, dt: torch.dtype) -> N.Pages:
+    _on(k_pages, dev, dt, "k_pages", 4)
+    _on(v_pages, dev, dt, "v_pages", 4)
+    n, h, ps, d = k_pages.shape
+    if v_pages.shape != k_pages.shape:
+        raise ValueError(f"fcenc: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} differ")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    return N.Pages(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], n, ps, h, d)
+
+
+@torch.library.custom_op("fcenc::kv_page_plan_", mutates_args=("kv_lens", "block_table", "free_pages", "free_count"))
+def kv_page_plan_(kv_lens: Tensor, new_lens: Tensor, finished: Optional[Tensor], block_table: Tensor, free_pages: Tensor,
+                  free_count: Tensor, page_size: int, rows: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """One step of a batch over a paged cache.  kv_lens int32 [B] tokens held, new_lens int32 [B] rows every request
+    brings, finished bool [B] or None (rows to empty first), block_table int32 [B][W], free_pages int32 [P] a stack of
+    free page ids of height free_count int32 [1], `rows` the rows of the step (sum of new_lens, or more) ->
+    (slots int64 [rows], cu_rows int32 [B + 1], granted bool [B]).  A row is granted when its tokens fit the table and the step's
+    rows and it needs no page, or the stack covers all that rows 0 .. b want: its pages move from the stack to the table and
+    kv_lens grows.  Slots are page * page_size + offset; -1 for refused requests and rows that belong to nobody."""
+    dev = kv_lens.device
+    _on(kv_lens, dev, torch.int32, "kv_lens", 1)
+    _on(new_lens, dev, torch.int32, "new_lens", 1)
+    _on(block_table, dev, torch.int32, "block_table", 2)
+    _on(free_pages, dev, torch.int32, "free_pages", 1)
+    _on(free_count, dev, torch.int32, "free_count", 1)
+    b, w = block_table.shape
+    if kv_lens.numel() != b or new_lens.numel() != b or free_count.numel() != 1:
+        raise ValueError("fcenc::kv_page_plan_: kv_lens and new_lens must hold one entry per table row, free_count one")
+    if finished is not None:
+        _on(finished, dev, torch.bool, "finished", 1)
+        if finished.numel() != b:
+            raise ValueError("fcenc::kv_page_plan_: finished must hold one entry per table row")
+    if rows < 0 or rows >= 2 ** 31 or b == 0 or w == 0 or free_pages.numel() == 0:
+        raise ValueError(f"fcenc::kv_page_plan_: {rows} rows, table {b} x {w}, {free_pages.numel()} pages")
+    slots = torch.empty((rows,), dtype=torch.int64, device=dev)
+    cu_rows = torch.empty((b + 1,), dtype=torch.int32, device=dev)
+    granted = torch.empty((b,), dtype=torch.bool, device=dev)
+    _launch(dev, N.lib().fcenc_page_plan, kv_lens.data_ptr(), new_lens.data_ptr(), N.ptr(finished), b, block_table.data_ptr(),
+            block_table.stride(0) if b > 1 else w, w, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size,
+            slots.data_ptr(), rows, cu_rows.data_ptr(), granted.data_ptr(), N.stream_of(kv_lens))
+    return slots, cu_rows, granted
+
+
+@kv_page_plan_.register_fake
+def _(kv_lens, new_lens, finished, block_table, free_pages, free_count, page_size, rows):
+    b = kv_lens.shape[0]
+    return (kv_lens.new_empty((rows,), dtype=torch.int64), kv_lens.new_empty((b + 1,)),
+            kv_lens.new_empty((b,), dtype=torch.bool))
+
+
+@torch.library.custom_op("fcenc::kv_page_write_", mutates_args=("k_pages", "v_pages"))
+def kv_page_write_(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots: Tensor) -> None:
+    """Rows of k and v [N][Hkv][D] (strided views of a fused projection are fine) into pages [P][Hkv][page_size][D] at
+    slots int64 [N]; a slot outside the pool (-1) is skipped.  Slots must differ: of two rows with one slot either may
+    stay."""
+    dev = k_pages.device
+    _on(k, dev, k_pages.dtype, "k", 3)
+    _on(v, dev, k_pages.dtype, "v", 3)
+    _on(slots, dev, torch.int64, "slots", 1)
+    pages = _pages(k_pages, v_pages, dev, k_pages.dtype)
+    n = slots.numel()
+    if tuple(k.shape) != (n, pages.kv_heads, pages.head_dim) or v.shape != k.shape:
+        raise ValueError(f"fcenc::kv_page_write_: k {tuple(k.shape)} and v {tuple(v.shape)} for {n} slots of {tuple(k_pages.shape)}")
+    if n == 0:
+        return
+    ks, vs = k.stride(), v.stride()
+    _launch(dev, N.lib().fcenc_page_write, _cdt(k), C.byref(pages), k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
+            slots.data_ptr(), n, N.stream_of(k))
+
+
+@kv_page_write_.register_fake
+def _(k, v, k_pages, v_pages, slots):
+    return None
+
+
+@torch.library.custom_op("fcenc::kv_page_attention", mutates_args=())
+def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor, kv_lens: Tensor, cu_rows: Tensor,
+                      scale: float, window: int = 0, sinks: int = 0, causal: bool = True, max_rows: int = 0) -> Tensor:
+    """Attention of a chunk of new rows over a paged cache that already holds the chunk's own tokens.  q [N][H][D]
+    (rows cu_rows[b] .. cu_rows[b+1] - 1 belong to request b), pages [P][Hkv][page_size][D], block_table int32 [B][W],
+    kv_lens int32 [B] -> [N][H][D].  The row at position p = kv_lens[b] - n + i sees token j < kv_lens[b] if
+    (not causal or j <= p) and (window == 0 or j > p - window or j < sinks).  Rows that see nothing, or belong to no request,
+    are zeros.  `max_rows` = the longest chunk, if the caller knows it (0: unknown): a hint for speed only."""
+    dev = q.device
+    _on(q, dev, q.dtype, "q", 3)
+    pages = _pages(k_pages, v_pages, dev, q.dtype)
+    _on(block_table, dev, torch.int32, "block_table", 2)
+    _on(kv_lens, dev, torch.int32, "kv_lens", 1)
+    _on(cu_rows, dev, torch.int32, "cu_rows", 1)
+    n, h, d = q.shape
+    b, w = block_table.shape
+    if d != pages.head_dim or kv_lens.numel() != b or cu_rows.numel() != b + 1:
+        raise ValueError(f"fcenc::kv_page_attention: q {tuple(q.shape)}, pages {tuple(k_pages.shape)}, {b} table rows, "
+                         f"{kv_lens.numel()} lengths, {cu_rows.numel()} row offsets")
+    dt = _cdt(q)
+    out = torch.empty((n, h, d), dtype=q.dtype, device=dev)
+    if n == 0:
+        return out
+    rows = N.PageRows(q.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_rows.data_ptr(), q.stride(0), q.stride(1),
+                      block_table.stride(0) if b > 1 else w, b, n, h, w, window, sinks, int(causal), max_rows, scale)
+    lib = N.lib()
+    need = lib.fcenc_page_attention_workspace_bytes(dt, C.byref(pages), C.byref(rows))
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    _launch(dev, lib.fcenc_page_attention, dt, C.byref(pages), C.byref(rows), out.data_ptr(), N.ptr(ws), need, N.stream_of(q))
+    return out
+
+
+@kv_page_attention.register_fake
+def _(q, k_pages, v_pages, block_table, kv_lens, cu_rows, scale, window=0, sinks=0, causal=True, max_rows=0):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("fcenc::sample_tokens", mutates_args=())
+def sample_tokens(logits: Tensor, u: Tensor, temperature: Optional[Tensor] = None, top_k: Optional[Tensor] = None,
+                  top_p: Optional[Tensor] = None, min_p: Optional[Tensor] = None) -> Tensor:
+    """One token per row of logits [R][V] (fp32 or bf16, V <= 2^18), drawn with u fp32 [R] in [0, 1) -> int32 [R].
+    Weights exp((x - max) / temperature); in the order of falling logits (equal ones by rising index) top_k int32 [R]
+    keeps the first k (<= 0: all), top_p fp32 [R] a token while the mass before it is below top_p times what top_k left
+    (>= 1: all), min_p fp32 [R] those of at least min_p times the largest weight (<= 0: all); the first is always kept.
+    The token is the first one, in index order, whose running mass exceeds u times the kept mass.  temperature <= 0
+    takes the first maximum.  NaN logits count as -inf; a row without any other gives -1."""
+    dev = logits.device
+    _on(logits, dev, logits.dtype, "logits", 2)
+    r, v = logits.shape
+    for nm, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                      ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is not None:
+            _on(t, dev, dt, nm, 1)
+            if t.numel() != r:
+                raise ValueError(f"fcenc::sample_tokens: {nm} must hold one value per row")
+    if v == 0:
+        raise ValueError("fcenc::sample_tokens: empty vocabulary")
+    tokens = torch.empty((r,), dtype=torch.int32, device=dev)
+    if r == 0:
+        return tokens
+    _launch(dev, N.lib().fcenc_sample_tokens, _cdt(logits), logits.data_ptr(), logits.stride(0) if r > 1 else v, r, v,
+            u.data_ptr(), N.ptr(temperature), N.ptr(top_k), N.ptr(top_p), N.ptr(min_p), tokens.data_ptr(), N.stream_of(logits))
+    return tokens
+
+
+@sample_tokens.register_fake
+def _(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    return logits.new_empty((logits.shape[0],), dtype=torch.int32)

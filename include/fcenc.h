@@ -453,6 +453,67 @@ typedef struct fcenc_mel_plan {
 int fcenc_mel_spectrogram(const fcenc_mel_plan* plan, const float* wave, long long ldw, const int64_t* lengths, int B,
                           int S, float* mel, int Tmax, int64_t* frames, void* stream);
 
+/* ---- pages of a key/value cache, attention over them, token sampling (serving many requests of different ages; no
+ * counterpart in the reference) ----
+ * A cache is a pool of n_pages pages of page_size slots (a power of two, 16 to 1024) for K and one for V.  A request
+ * that holds n tokens has its page ids in entries 0 .. ceil(n / page_size) - 1 of its row of the block table
+ * (int32 [B][table_row], the first table_width columns used); token j is slot j % page_size of page j / page_size.
+ *
+ * fcenc_page_plan: one step of a batch.  Row b brings new_lens[b] rows.  Rows with finished[b] != 0 (may be null) first
+ * push their pages on the stack free_pages[0 .. *free_count) and start from 0 tokens.  A row is granted when its
+ * tokens fit the table and cu_rows[b + 1] <= rows, and it needs no page or all pages wanted by rows 0 .. b are there;
+ * its pages come off the stack into the table, kv_lens[b] grows by new_lens[b], and
+ * slots[cu_rows[b] + i] = page * page_size + offset of its i-th row.  Rows of refused requests and rows at and behind
+ * cu_rows[B] get slot -1; a refused row keeps its length.  cu_rows int32 [B + 1] = running sum of new_lens,
+ * granted uint8 [B], slots int64 [rows]; kv_lens, block_table, free_pages (pool_pages entries) and free_count are
+ * updated in place.  Negative lengths count as 0.
+ *
+ * fcenc_page_write: rows of k and v (element strides k_row, k_head, ..., head_dim contiguous) to their slots; a slot
+ * outside the pool is skipped.  Two rows with one slot leave either of them there.
+ *
+ * fcenc_page_attention: request b has rows cu_rows[b] .. cu_rows[b + 1] - 1 of q (n of them) at positions
+ * kv_lens[b] - n + i, its tokens (those rows' own K and V among them) already in the pages.  A row at position p sees
+ * token j < kv_lens[b] if (not causal or j <= p) and (window == 0 or j > p - window or j < sinks); tokens of pages
+ * whose id is outside the pool are seen by nobody.  out [rows][heads][head_dim] (dense); rows that see nothing and rows that
+ * belong to no request are zeros.  Query head h reads kv head h / (heads / kv_heads).  head_dim <= 128 and a
+ * multiple of 8; all strides in elements, multiples of 16 bytes; scale > 0.  max_rows: the longest chunk of the batch if
+ * the caller knows it, else 0 -- it chooses kernels and never changes what is computed.  The workspace (size from
+ * fcenc_page_attention_workspace_bytes, may be 0) belongs to one call at a time.
+ *
+ * fcenc_sample_tokens: one token per row of logits [rows][row_stride] (vocab <= 2^18 used).  With weights
+ * w_i = exp((x_i - max) / temperature) and the order of falling logits (equal ones by rising index): top_k keeps the
+ * first k (<= 0: all), top_p keeps a token while the mass before it is below top_p times what top_k left (>= 1:
+ * all), min_p keeps w_i >= min_p; the first is always kept.  u in [0, 1) picks, in index order, the first token whose
+ * running sum exceeds u times the sum.  temperature <= 0: the first maximum.  NaN logits count as -inf; a row of
+ * nothing but -inf gives -1.  Parameters are per row; null pointers mean temperature 1 and no filter. */
+typedef struct fcenc_pages {
+  void* k;
+  void* v;
+  long long k_page, k_head, k_slot, v_page, v_head, v_slot;   /* strides in elements */
+  int n_pages, page_size, kv_heads, head_dim;
+} fcenc_pages;
+typedef struct fcenc_page_rows {
+  const void* q;
+  const int32_t* block_table;
+  const int32_t* kv_lens;
+  const int32_t* cu_rows;
+  long long q_row, q_head, table_row;
+  int batch, rows, heads, table_width;
+  int window, sinks, causal, max_rows;
+  float scale;
+} fcenc_page_rows;
+int fcenc_page_plan(int32_t* kv_lens, const int32_t* new_lens, const uint8_t* finished, int B, int32_t* block_table,
+                    long long table_row, int table_width, int32_t* free_pages, int32_t* free_count, int pool_pages,
+                    int page_size, int64_t* slots, int rows, int32_t* cu_rows, uint8_t* granted, void* stream);
+int fcenc_page_write(int dtype, const fcenc_pages* pages, const void* k, const void* v, long long k_row, long long k_head,
+                     long long v_row, long long v_head, const int64_t* slots, int rows, void* stream);
+size_t fcenc_page_attention_workspace_bytes(int dtype, const fcenc_pages* pages, const fcenc_page_rows* rows);
+int fcenc_page_attention(int dtype, const fcenc_pages* pages, const fcenc_page_rows* rows, void* out, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int fcenc_sample_tokens(int dtype, const void* logits, long long row_stride, int rows, int vocab, const float* u,
+                        const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                        int32_t* tokens, void* stream);
+
 /* frames after subsampling and the padded frame count the kernels use (multiple of 64) */
 int fcenc_out_frames(int T);
 int fcenc_padded_frames(int T);
