@@ -35,6 +35,17 @@ constexpr uint32_t OOB = 0xF0000000u;       // an offset outside every descripto
 constexpr int MAX_SPLITS = 64;
 constexpr int STEP_WAVES = 4;
 constexpr int STEP_ROWS = 16;
+constexpr int CHUNK_ROWS = 128;             // rows of a tile of the chunk kernel
+constexpr int CHUNK_MIN = 32;               // requests with more rows (times heads per kv head) than this are its share
+
+// How a launch divides the work: `pieces` of the key axis here, `ws_pieces` in the workspace; `share` 0: every request,
+// 1: those of up to CHUNK_MIN rows and the rows behind the last request, 2: the longer ones.
+struct Split {
+  int gc = 1, hchunks = 1, tt = 1, pieces = 1, ws_pieces = 1, share = 0;
+};
+
+// Partial results of a split key axis: (m, l) of every (row, head, piece), then the unnormalised sums.
+__device__ __host__ __forceinline__ long long ws_sums(long long rows, int pieces) { return (2 * rows * pieces + 3) & ~3ll; }
 
 struct TileInfo {
   int b, t0, n, c0, kv;                      // request (B: rows behind the last one), first row, rows, offset, tokens
@@ -63,6 +74,10 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, int t
     ti.kv = kv < 0 ? 0 : (kv > cap ? cap : kv);
   }
   return true;
+}
+
+__device__ __forceinline__ bool is_chunk(const PageAttnArgs& a, const TileInfo& ti, int group) {
+  return ti.b < a.B && (long long)ti.n * group > CHUNK_MIN;
 }
 
 // V^T fragment of a [32 tokens][DP] tile in LDS: element j of lane (g, r) is V[token 16 (j >> 2) + 4 g + (j & 3)][dim 16 db + r]
@@ -139,7 +154,7 @@ struct StepTile {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 ? 1 : 2))
-    page_attn_step_kernel(const PageAttnArgs a, int gc, int hchunks, int tt, int splits) {
+    page_attn_step_kernel(const PageAttnArgs a, const Split sp) {
   using TL = StepTile<T, DP>;
   using Frag = typename Traits<T>::Frag;
   constexpr int ROWB = TL::ROWB, CPR = TL::CPR, ES = (int)sizeof(T);
@@ -149,12 +164,13 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int kvh = blockIdx.y / hchunks, hc = blockIdx.y - kvh * hchunks;
-  const int split = blockIdx.z;
+  const int gc = sp.gc, tt = sp.tt, split = blockIdx.z;
+  const int kvh = blockIdx.y / sp.hchunks, hc = blockIdx.y - kvh * sp.hchunks;
   const int group = a.heads / a.kv_heads;
 
   TileInfo ti;
   if (!find_tile(a, blockIdx.x, tt, ti)) return;
+  if (sp.share == 1 && is_chunk(a, ti, group)) return;
   const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
   const int last = first + (ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt) - 1;
   int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
@@ -166,7 +182,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   int sb = ((sinks < hi ? sinks : hi) + 31) >> 5;
   sb = sb < lob ? sb : lob;
   const int count = hi > 0 ? sb + ((hi + 31) >> 5) - lob : 0;
-  const int i0 = (int)((long long)count * split / splits), i1 = (int)((long long)count * (split + 1) / splits);
+  const int i0 = (int)((long long)count * split / sp.pieces), i1 = (int)((long long)count * (split + 1) / sp.pieces);
 
   // this lane's row of the tile
   const int rt = r / gc, rh = hc * gc + r - rt * gc;
@@ -325,7 +341,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
     for (int d = 0; d < DPT; ++d) acc[d] += src[d] * f;
   }
   const long long orow = (long long)(ti.c0 + ti.t0 + ort) * a.heads + kvh * group + orh;
-  if (splits == 1) {
+  if (sp.ws_pieces == 1) {
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);       // NaN stays NaN
     T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
 #pragma unroll
@@ -333,11 +349,317 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
       if (d0 + d < a.dim) store_row(o + d0 + d, acc[d] * inv);
   } else {
     const long long rows = (long long)a.rows * a.heads;
-    float* o = a.ws + 2 * rows * splits + (orow * splits + split) * a.dim;
+    float* o = a.ws + ws_sums(rows, sp.ws_pieces) + (orow * sp.ws_pieces + split) * a.dim;
 #pragma unroll
     for (int d = 0; d < DPT; ++d)
       if (d0 + d < a.dim) o[d0 + d] = acc[d];
-    if ((tid & 15) == 0) reinterpret_cast<float2*>(a.ws)[orow * splits + split] = float2{m, l};
+    if ((tid & 15) == 0) {
+      float2* out = reinterpret_cast<float2*>(a.ws) + orow * sp.ws_pieces;
+      out[split] = float2{m, l};
+      if (split == 0)
+        for (int i = sp.pieces; i < sp.ws_pieces; ++i) out[i] = float2{-INFINITY, 0.f};
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Tiles of up to 128 rows: chunks and prompts.  Four waves of 32 rows share each K / V tile of 64 tokens through LDS;
+// 32x32 MFMAs, so a wave reads a fragment once for 32 rows and a row's statistics need one exchange between the two
+// halves of the wave.  A tile is loaded into registers (wave w: tokens 16w .. 16w + 15, one page lookup) while the one
+// before it is multiplied, then written to LDS.
+//
+// C layout of a 32x32 product: lane (h = lane / 32, c = lane % 32), register i: row 8 (i / 4) + 4 h + i % 4, column c.  With
+// rows = tokens, registers 8 s .. 8 s + 7 are the eight tokens {4 h + 0..3, 8 + 4 h + 0..3} of 16-token step s: the k
+// elements of lane half h of the next product, whose V^T fragment is read in that order.
+// ---------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void mma32(f32x16& acc, const bf16x8& a, const bf16x8& b) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma32(f32x16& acc, const f32x8& a, const f32x8& b) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.lo[j], b.lo[j], acc, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.hi[j], b.hi[j], acc, 0, 0, 0);
+}
+
+template <typename T, int DP>
+struct ChunkTile {
+  static constexpr int ROWB = DP * (int)sizeof(T);
+  static constexpr int CPR = ROWB / 16;
+  static constexpr int KT = 64;                                  // tokens of a tile
+  static constexpr int V_OFF = KT * ROWB;
+  static constexpr int OK_OFF = 2 * KT * ROWB;                   // 4 flags: the page of every 16 tokens exists
+  static constexpr int STAGE = OK_OFF + 16;
+  static constexpr int NST = sizeof(T) == 2 ? 2 : 1;             // fp32 tiles are twice as large: one stage, two barriers
+  static constexpr int BYTES = NST * STAGE;
+};
+
+// K: 8 lanes that read one chunk of 8 rows hit 8 different ones.  V: the 4 rows x 32 bytes of a transposing read lie in
+// 128 different bytes.
+template <int ROWB>
+__device__ __forceinline__ uint32_t k_off(int row, int ch) { return (uint32_t)(row * ROWB + ((ch ^ (row & 7)) << 4)); }
+template <int ROWB>
+__device__ __forceinline__ uint32_t v_off(int row, int ch, bf16) {
+  return (uint32_t)(row * ROWB + ((ch ^ ((row & (ROWB >= 256 ? 7 : 3)) << 1)) << 4));
+}
+template <int ROWB>
+__device__ __forceinline__ uint32_t v_off(int row, int ch, float) { return k_off<ROWB>(row, ch); }
+
+template <int ROWB>
+__device__ __forceinline__ bf16x8 k_frag32(const char* kt, int row, int ks, int h, bf16) {
+  return *reinterpret_cast<const bf16x8*>(kt + k_off<ROWB>(row, 2 * ks + h));
+}
+template <int ROWB>
+__device__ __forceinline__ f32x8 k_frag32(const char* kt, int row, int ks, int h, float) {
+  f32x8 f;
+  f.lo = *reinterpret_cast<const f32x4*>(kt + k_off<ROWB>(row, 4 * ks + 2 * h));
+  f.hi = *reinterpret_cast<const f32x4*>(kt + k_off<ROWB>(row, 4 * ks + 2 * h + 1));
+  return f;
+}
+// V^T of dims 32 dt .. + 31, 16-token step s: element j of lane (h, c) is V[16 s + 8 (j >> 2) + 4 h + (j & 3)][32 dt + c]
+template <int ROWB>
+__device__ __forceinline__ bf16x8 v_frag32(const char* vt, int dt, int s, int lane, bf16) {
+  using lds_bf16x4 = __attribute__((address_space(3))) bf16x4;
+  const int h = lane >> 5, half = (lane >> 4) & 1, r = lane & 15;
+  bf16x8 f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int key = 16 * s + 8 * u + 4 * h + (r >> 2);
+    const char* p = vt + v_off<ROWB>(key, 4 * dt + 2 * half + ((r & 3) >> 1), bf16{}) + 8 * (r & 1);
+    const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p));
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f[4 * u + q] = v[q];
+  }
+  return f;
+}
+template <int ROWB>
+__device__ __forceinline__ f32x8 v_frag32(const char* vt, int dt, int s, int lane, float) {
+  const int h = lane >> 5, d = 32 * dt + (lane & 31);
+  f32x8 f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int key = 16 * s + 8 * (j >> 2) + 4 * h + (j & 3);
+    const float v = *reinterpret_cast<const float*>(vt + v_off<ROWB>(key, d >> 2, float{}) + 4 * (d & 3));
+    if (j < 4) f.lo[j] = v; else f.hi[j - 4] = v;
+  }
+  return f;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
+    page_attn_chunk_kernel(const PageAttnArgs a, const Split sp) {
+  using TL = ChunkTile<T, DP>;
+  using Frag = typename Traits<T>::Frag;
+  constexpr int ROWB = TL::ROWB, CPR = TL::CPR, ES = (int)sizeof(T);
+  constexpr int KS = DP / 16, NDT = DP / 32, NL = CPR / 4, RPI = 64 / CPR;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uniform(tid >> 6);
+  const int h = lane >> 5, c = lane & 31;
+  // workgroups of one kv head are dispatched to one XCD where the number of kv heads allows it (their tiles read the same
+  // keys), long tiles (the late rows of a causal chunk) first
+  const int columns = a.kv_heads * sp.hchunks;
+  const int tile = (int)((gridDim.x - 1 - blockIdx.x) / columns), column = (int)(blockIdx.x % columns);
+  const int kvh = column / sp.hchunks, hc = column - kvh * sp.hchunks;
+  const int gc = sp.gc, tt = sp.tt, split = blockIdx.y;
+  const int group = a.heads / a.kv_heads;
+
+  TileInfo ti;
+  if (!find_tile(a, tile, tt, ti)) return;
+  if (sp.share == 2 && !is_chunk(a, ti, group)) return;
+  const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
+  const int live_tt = ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt;
+  const int last = first + live_tt - 1;
+  int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
+  if (ti.b == a.B || hi < 0) hi = 0;
+  int lo = a.window > 0 ? first - a.window + 1 : 0;
+  lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
+  const int sinks = a.window > 0 ? a.sinks : 0;
+  const int lot = lo >> 6;
+  int sb = ((sinks < hi ? sinks : hi) + 63) >> 6;
+  sb = sb < lot ? sb : lot;
+  const int count = hi > 0 ? sb + ((hi + 63) >> 6) - lot : 0;
+  const int i0 = (int)((long long)count * split / sp.pieces), i1 = (int)((long long)count * (split + 1) / sp.pieces);
+
+  // this lane's row and this wave's rows
+  const int R = 32 * wave + c;
+  const int rt = R / gc, rh = hc * gc + R - rt * gc;
+  const bool live = rt < live_tt && rh < group;
+  const int pos = first + rt;
+  const int see_hi = a.causal ? pos : ti.kv - 1;
+  const int see_lo = a.window > 0 ? pos - a.window + 1 : 0;
+  const int wt0 = (32 * wave) / gc;
+  int wt1 = (32 * wave + 31) / gc;
+  wt1 = wt1 < live_tt - 1 ? wt1 : live_tt - 1;
+  const bool busy = wt0 <= wt1;
+  const int wfirst = first + wt0, wlast = first + wt1;       // positions of the wave's first and last row
+
+  Frag q[KS];
+  {
+    const char* qrow = a.q + (long long)(ti.c0 + ti.t0 + (live ? rt : 0)) * a.q_row + (long long)(kvh * group + (live ? rh : 0)) * a.q_head;
+    const __amdgpu_buffer_rsrc_t none = buffer_of(nullptr, 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      q[ks] = load_frag(none, OOB, T{});
+      if (live && 16 * ks + 8 * h < a.dim) q[ks] = *reinterpret_cast<const Frag*>(qrow + (16 * ks + 8 * h) * ES);
+    }
+  }
+
+  f32x16 ot[NDT];
+#pragma unroll
+  for (int i = 0; i < NDT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ot[i][e] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;                      // m in units of the raw scores
+  const float cs = a.scale * kLog2e;
+  const int32_t* trow = a.table + (long long)(ti.b < a.B ? ti.b : 0) * a.table_row;
+  const char* kbase = a.k + kvh * a.k_head;
+  const char* vbase = a.v + kvh * a.v_head;
+
+  u32x4 kr[NL], vr[NL];
+  int ok = 0;
+  auto tile_of = [&](int i) { return i < sb ? i : lot + i - sb; };
+  auto fetch = [&](int i) {
+    const int tok0 = tile_of(i) * 64 + 16 * wave;
+    int left = hi - tok0;
+    left = left > 16 ? 16 : left;
+    int page = -1;
+    if (left > 0) page = uniform(trow[tok0 >> a.shift]);
+    const bool good = page >= 0 && page < a.n_pages;
+    ok = good || left <= 0;
+    const int slot0 = tok0 & ((1 << a.shift) - 1);
+    const char* kp = kbase + (long long)(good ? page : 0) * a.k_page + (long long)slot0 * a.k_slot;
+    const char* vp = vbase + (long long)(good ? page : 0) * a.v_page + (long long)slot0 * a.v_slot;
+    const __amdgpu_buffer_rsrc_t kd = buffer_of(kp, good ? (left - 1) * a.k_slot + a.dim * ES : 0);
+    const __amdgpu_buffer_rsrc_t vd = buffer_of(vp, good ? (left - 1) * a.v_slot + a.dim * ES : 0);
+#pragma unroll
+    for (int v = 0; v < NL; ++v) {
+      const int row = v * RPI + lane / CPR, ch = lane % CPR;
+      // nobody sees the tokens between the sinks and the window
+      const bool dead = ch * 16 >= a.dim * ES || (tok0 + row < lo && tok0 + row >= sinks);
+      kr[v] = __builtin_amdgcn_raw_buffer_load_b128(kd, (int)(dead ? OOB : (uint32_t)(row * a.k_slot + ch * 16)), 0, 0);
+      vr[v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(dead ? OOB : (uint32_t)(row * a.v_slot + ch * 16)), 0, 0);
+    }
+  };
+  auto commit = [&](char* st) {
+#pragma unroll
+    for (int v = 0; v < NL; ++v) {
+      const int row = 16 * wave + v * RPI + lane / CPR, ch = lane % CPR;
+      *reinterpret_cast<u32x4*>(st + k_off<ROWB>(row, ch)) = kr[v];
+      *reinterpret_cast<u32x4*>(st + TL::V_OFF + v_off<ROWB>(row, ch, T{})) = vr[v];
+    }
+    if (lane == 0) reinterpret_cast<int*>(st + TL::OK_OFF)[wave] = ok;
+  };
+
+  if (i0 < i1) {
+    fetch(i0);
+    commit(smem);
+  }
+  for (int i = i0; i < i1; ++i) {
+    char* st = smem + (TL::NST == 2 ? (i - i0) & 1 : 0) * TL::STAGE;
+    __syncthreads();
+    const bool more = i + 1 < i1;
+    if (more) fetch(i + 1);
+    const int j0 = tile_of(i) * 64;
+    // a wave skips tiles that none of its rows sees
+    bool sees = busy && (!a.causal || j0 <= wlast);
+    if (a.window > 0) sees = sees && (j0 + 63 >= wfirst - a.window + 1 || j0 < sinks);
+    if (sees) {
+      const u32x4 okv = *reinterpret_cast<const u32x4*>(st + TL::OK_OFF);
+      f32x16 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) mma32(s[t], k_frag32<ROWB>(st, 32 * t + c, ks, h, T{}), q[ks]);
+      }
+      bool inside = uniform(okv[0] & okv[1] & okv[2] & okv[3]) && j0 + 63 <= (a.causal ? wfirst : ti.kv - 1);
+      if (a.window > 0) inside = inside && (j0 >= wlast - a.window + 1 || j0 + 63 < sinks);
+      if (!inside) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = j0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+            const bool see = okv[2 * t + (e >> 3)] && j <= see_hi && (j >= see_lo || j < sinks);
+            s[t][e] = see ? s[t][e] : -INFINITY;
+          }
+      }
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, s[t][e]);
+      {
+        float x, y;
+        swap_halves32(tmax, x, y);
+        tmax = fmaxf(x, y);
+      }
+      const float m_new = fmaxf(m_run, tmax);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new * cs;
+      if (__any(m_new > m_run)) {                            // the maximum seldom moves once a few tiles have gone by
+        const float alpha = __builtin_amdgcn_exp2f(m_run * cs - m_use);
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) ot[dt] *= alpha;
+        m_run = m_new;
+      }
+      float psum = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        float pk[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pk[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + e], cs, -m_use));
+          psum += pk[e];
+        }
+        // rounded to the storage type for the product; the sum is not
+        const Frag pf = p_frag(pk, T{});
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) mma32(ot[dt], v_frag32<ROWB>(st + TL::V_OFF, dt, u, lane, T{}), pf);
+      }
+      l_run += psum;
+    }
+    if (more) {
+      if (TL::NST == 1) __syncthreads();
+      commit(smem + (TL::NST == 2 ? (i + 1 - i0) & 1 : 0) * TL::STAGE);
+    }
+  }
+
+  {
+    float x, y;
+    swap_halves32(l_run, x, y);
+    l_run = x + y;
+  }
+  if (!live) return;
+  const long long orow = (long long)(ti.c0 + ti.t0 + rt) * a.heads + kvh * group + rh;
+  if (sp.ws_pieces == 1) {
+    const float inv = l_run > 0.f ? 1.0f / l_run : (l_run == 0.f ? 0.f : l_run);       // NaN stays NaN
+    T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 32 * dt + 8 * e + 4 * h;
+        if (d < a.dim) store4(o + d, f32x4{ot[dt][4 * e], ot[dt][4 * e + 1], ot[dt][4 * e + 2], ot[dt][4 * e + 3]} * inv);
+      }
+  } else {
+    const long long rows = (long long)a.rows * a.heads;
+    float* o = a.ws + ws_sums(rows, sp.ws_pieces) + (orow * sp.ws_pieces + split) * a.dim;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 32 * dt + 8 * e + 4 * h;
+        if (d < a.dim) store4(o + d, f32x4{ot[dt][4 * e], ot[dt][4 * e + 1], ot[dt][4 * e + 2], ot[dt][4 * e + 3]});
+      }
+    if (h == 0) {
+      float2* out = reinterpret_cast<float2*>(a.ws) + orow * sp.ws_pieces;
+      out[split] = float2{m_run * cs, l_run};                // the join works in base-2 exponents
+      if (split == 0)
+        for (int i = sp.pieces; i < sp.ws_pieces; ++i) out[i] = float2{-INFINITY, 0.f};
+    }
   }
 }
 
@@ -358,7 +680,7 @@ __global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs 
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
   const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  const float* src = a.ws + 2 * rows * splits + row * splits * a.dim;
+  const float* src = a.ws + ws_sums(rows, splits) + row * splits * a.dim;
   float acc[2] = {0.f, 0.f};
   for (int s = 0; s < splits; ++s) {
     const float w = __shfl(f, s);
@@ -375,32 +697,63 @@ __global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs 
 // ---------------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------------
-struct StepPlan {
-  int gc, hchunks, tt, tiles, splits;
+struct Plan {
+  Split step, chunk;
+  int step_tiles = 0, chunk_tiles = 0;                       // chunk_tiles 0: not launched
+  int pieces = 1;
 };
 
-StepPlan step_plan(const PageAttnArgs& a) {
-  StepPlan s;
-  const int group = a.heads / a.kv_heads;
-  s.gc = group < STEP_ROWS ? group : STEP_ROWS;
-  s.hchunks = (group + s.gc - 1) / s.gc;
-  s.tt = STEP_ROWS / s.gc;
-  s.tiles = a.rows / s.tt + a.B + 1;
-  // workgroups that have work, and how many pieces of the key axis fill the chip with four per CU; a piece is at
-  // least 256 tokens long for the longest request that the table can describe
-  const long long full = (a.rows + s.tt - 1) / s.tt, some = a.rows < a.B ? a.rows : a.B;
-  const long long busy = (full > some ? full : some) * a.kv_heads * s.hchunks;
+// pieces of the key axis that give a launch `want` workgroups, none shorter than `least` tokens for the longest request
+// that the table can describe
+int pieces_for(const PageAttnArgs& a, long long busy, long long want, int least) {
   long long longest = (long long)a.width << a.shift;
-  if (a.window > 0 && (long long)a.window + a.sinks + s.tt + 64 < longest) longest = (long long)a.window + a.sinks + s.tt + 64;
-  long long sp = busy > 0 ? 1024 / busy : 1;
-  if (sp > longest / 256) sp = longest / 256;
-  if (sp > MAX_SPLITS) sp = MAX_SPLITS;
-  s.splits = sp < 1 ? 1 : (int)sp;
-  return s;
+  const long long seen = (long long)a.window + a.sinks + CHUNK_ROWS;
+  if (a.window > 0 && seen < longest) longest = seen;
+  long long n = want / (busy > 0 ? busy : 1);
+  if (n > longest / least) n = longest / least;
+  if (n > MAX_SPLITS) n = MAX_SPLITS;
+  return n < 1 ? 1 : (int)n;
 }
 
-size_t split_bytes(const PageAttnArgs& a, int splits) {
-  return splits > 1 ? (size_t)a.rows * a.heads * splits * (a.dim + 2) * sizeof(float) : 0;
+Plan make_plan(const PageAttnArgs& a) {
+  Plan p;
+  const int group = a.heads / a.kv_heads;
+  const long long longest = a.max_rows > 0 && a.max_rows < a.rows ? a.max_rows : a.rows;      // rows of one request
+  const bool chunks = longest * group > CHUNK_MIN;
+  // without a hint a batch of as many rows as requests is taken for single tokens (the chunk kernel would find nothing)
+  const bool only_steps = !chunks || (a.max_rows == 0 && a.rows <= a.B);
+  const long long some = a.rows < a.B ? a.rows : a.B;
+  {
+    Split& s = p.step;
+    s.gc = group < STEP_ROWS ? group : STEP_ROWS;
+    s.hchunks = (group + s.gc - 1) / s.gc;
+    s.tt = STEP_ROWS / s.gc;
+    s.share = only_steps ? 0 : 1;
+    p.step_tiles = a.rows / s.tt + a.B + 1;
+    const long long full = only_steps ? (a.rows + s.tt - 1) / s.tt : some;
+    s.pieces = pieces_for(a, (full > some ? full : some) * a.kv_heads * s.hchunks, 1024, 256);
+  }
+  p.pieces = p.step.pieces;
+  if (!only_steps) {
+    Split& s = p.chunk;
+    s.gc = group < CHUNK_ROWS ? group : CHUNK_ROWS;
+    s.hchunks = (group + s.gc - 1) / s.gc;
+    s.tt = CHUNK_ROWS / s.gc;
+    s.share = 2;
+    p.chunk_tiles = a.rows / s.tt + a.B + 1;
+    s.pieces = pieces_for(a, (a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 1024, 512);
+    if (s.pieces > p.pieces) p.pieces = s.pieces;
+  }
+  p.step.ws_pieces = p.chunk.ws_pieces = p.pieces;
+  return p;
+}
+
+long long chunk_grid(const PageAttnArgs& a, const Plan& p) { return (long long)p.chunk_tiles * a.kv_heads * p.chunk.hchunks; }
+
+size_t split_bytes(const PageAttnArgs& a, int pieces) {
+  if (pieces <= 1) return 0;
+  const long long rows = (long long)a.rows * a.heads;
+  return (size_t)(ws_sums(rows, pieces) + rows * pieces * a.dim) * sizeof(float);
 }
 
 int check_args(int dtype, const PageAttnArgs& a) {
@@ -422,14 +775,20 @@ int check_args(int dtype, const PageAttnArgs& a) {
 }
 
 template <typename T, int DP>
-int run_step(const PageAttnArgs& a, const StepPlan& s, hipStream_t stream) {
-  using TL = StepTile<T, DP>;
-  auto k = page_attn_step_kernel<T, DP>;
-  if (reserve_lds(reinterpret_cast<const void*>(k), TL::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", TL::BYTES);
-  k<<<dim3(s.tiles, a.kv_heads * s.hchunks, s.splits), 64 * STEP_WAVES, TL::BYTES, stream>>>(a, s.gc, s.hchunks, s.tt, s.splits);
-  if (s.splits > 1) {
+int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
+  using ST = StepTile<T, DP>;
+  using CT = ChunkTile<T, DP>;
+  auto sk = page_attn_step_kernel<T, DP>;
+  auto ck = page_attn_chunk_kernel<T, DP>;
+  if (p.chunk_tiles > 0) {
+    if (reserve_lds(reinterpret_cast<const void*>(ck), CT::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", CT::BYTES);
+    ck<<<dim3((unsigned)chunk_grid(a, p), p.chunk.pieces), 256, CT::BYTES, stream>>>(a, p.chunk);
+  }
+  if (reserve_lds(reinterpret_cast<const void*>(sk), ST::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", ST::BYTES);
+  sk<<<dim3(p.step_tiles, a.kv_heads * p.step.hchunks, p.step.pieces), 64 * STEP_WAVES, ST::BYTES, stream>>>(a, p.step);
+  if (p.pieces > 1) {
     const long long rows = (long long)a.rows * a.heads;
-    page_attn_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(a, s.splits);
+    page_attn_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(a, p.pieces);
   }
   return check_launch("page_attention");
 }
@@ -438,19 +797,20 @@ int run_step(const PageAttnArgs& a, const StepPlan& s, hipStream_t stream) {
 
 size_t page_attention_workspace_bytes(int dtype, const PageAttnArgs& a) {
   if (check_args(dtype, a) != 0) return 0;
-  return split_bytes(a, step_plan(a).splits);
+  return split_bytes(a, make_plan(a).pieces);
 }
 
 int launch_page_attention(int dtype, const PageAttnArgs& a, size_t ws_bytes, hipStream_t stream) {
   if (check_args(dtype, a) != 0) return -1;
   if (a.rows == 0) return 0;
   if (!a.q || !a.k || !a.v || !a.table || !a.kv_lens || !a.cu_rows || !a.out) return fail("page_attention: null operand");
-  if ((uintptr_t)a.q % 16 || (uintptr_t)a.k % 16 || (uintptr_t)a.v % 16) return fail("page_attention: operands must be 16-byte aligned");
-  const StepPlan s = step_plan(a);
-  const size_t need = split_bytes(a, s.splits);
+  if ((uintptr_t)a.q % 16 || (uintptr_t)a.k % 16 || (uintptr_t)a.v % 16 || (uintptr_t)a.out % 16) return fail("page_attention: operands must be 16-byte aligned");
+  const Plan p = make_plan(a);
+  const size_t need = split_bytes(a, p.pieces);
   if (need > 0 && (!a.ws || ws_bytes < need || (uintptr_t)a.ws % 16)) return fail("page_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  if (dtype == DT_BF16) return a.dim <= 64 ? run_step<bf16, 64>(a, s, stream) : run_step<bf16, 128>(a, s, stream);
-  return a.dim <= 64 ? run_step<float, 64>(a, s, stream) : run_step<float, 128>(a, s, stream);
+  if (chunk_grid(a, p) > 0x7fffffffll || (long long)a.kv_heads * p.step.hchunks > 65535) return fail("page_attention: too many rows or heads");
+  if (dtype == DT_BF16) return a.dim <= 64 ? run<bf16, 64>(a, p, stream) : run<bf16, 128>(a, p, stream);
+  return a.dim <= 64 ? run<float, 64>(a, p, stream) : run<float, 128>(a, p, stream);
 }
 
 }  // namespace fcenc

@@ -24,6 +24,7 @@ constexpr int PLAN_WAVES = PLAN_THREADS / 64;
 // Steps with up to this many rows (and PLAN_THREADS requests) find their slots in the planning workgroup itself, out of
 // LDS; longer ones leave them to a second launch over all CUs.
 constexpr int PLAN_INLINE_ROWS = 4 * PLAN_THREADS;
+constexpr int OWN_PAGES = 4;
 
 __device__ __forceinline__ long long wave_scan(long long v, int lane) {      // inclusive
 #pragma unroll
@@ -34,17 +35,20 @@ __device__ __forceinline__ long long wave_scan(long long v, int lane) {      // 
   return v;
 }
 
-// inclusive prefix sum of one value per thread; `total` receives the sum.  `part` holds PLAN_WAVES values.
-__device__ __forceinline__ long long block_scan(long long v, long long* part, long long& total) {
+// inclusive prefix sum of one value per thread; `total` receives the sum.  `part` holds a value per wave.
+__device__ __forceinline__ long long block_scan(long long v, long long* part, int waves, long long& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const long long incl = wave_scan(v, lane);
+  if (waves == 1) {
+    total = __shfl(incl, 63);
+    return incl;
+  }
   __syncthreads();                       // the last use of `part` is over
   if (lane == 63) part[wave] = incl;
   __syncthreads();
   long long base = 0;
   total = 0;
-#pragma unroll 2
-  for (int w = 0; w < PLAN_WAVES; ++w) {
+  for (int w = 0; w < waves; ++w) {
     if (w < wave) base += part[w];
     total += part[w];
   }
@@ -58,21 +62,20 @@ __device__ __forceinline__ long long slot_of(const int32_t* row, int pos, int sh
 }
 
 // One workgroup: a plan is a chain of prefix sums over a few hundred requests, bound by latency, and one workgroup
-// needs no hand-over between CUs.  Waves fill the table rows of their requests.
+// needs no hand-over between CUs.  It has a thread per request or row up to PLAN_THREADS; with one wave no scan waits at a barrier.
+// A thread moves up to OWN_PAGES pages of its request by itself, a wave those of a longer one together.
 __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanArgs a, int inline_slots) {
   __shared__ long long part[PLAN_WAVES];
-  __shared__ int s_kv[PLAN_THREADS];                 // length before the step (0 for rows that finished)
+  __shared__ int s_kv[PLAN_THREADS];                 // length before the step (0 for rows that finished), -1 if refused
   __shared__ int s_cu[PLAN_THREADS + 1];
-  __shared__ int s_take[PLAN_THREADS];               // pages handed out before this row
-  __shared__ int s_need[PLAN_THREADS];               // pages it gets; -1 if refused
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x, waves = threads >> 6;
   const int cap = a.width << a.shift;                // the longest request the table can describe
   int top = *a.free_count;
   top = top < 0 ? 0 : (top > a.pool ? a.pool : top);
 
   // ---- 1. rows that finished ----
   if (a.finished) {
-    for (int b0 = 0; b0 < a.B; b0 += PLAN_THREADS) {
+    for (int b0 = 0; b0 < a.B; b0 += threads) {
       const int b = b0 + tid;
       int count = 0;
       if (b < a.B && a.finished[b]) {
@@ -81,21 +84,17 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanA
         count = pages_of(kv, a.shift);
       }
       long long total;
-      const long long incl = block_scan(count, part, total);
-      s_need[tid] = count;
-      const long long first = top + incl - count;
-      s_take[tid] = first > a.pool ? a.pool : (int)first;
-      __syncthreads();
-      const int rows = a.B - b0 < PLAN_THREADS ? a.B - b0 : PLAN_THREADS;
-      for (int i = wave; i < rows; i += PLAN_WAVES) {
-        const int32_t* row = a.table + (size_t)(b0 + i) * a.table_row;
-        const int n = s_need[i], at = s_take[i];
+      const long long first = top + block_scan(count, part, waves, total) - count;
+      const int at = first > a.pool ? a.pool : (int)first;
+      for (unsigned long long m = __ballot(count > 0); m; m &= m - 1) {
+        const int i = __ffsll(m) - 1;
+        const int n = __shfl(count, i), to = __shfl(at, i);
+        const int32_t* row = a.table + (size_t)(b - lane + i) * a.table_row;
         for (int c = lane; c < n; c += 64)
-          if (c < a.pool - at) a.free_pages[at + c] = row[c];     // a pool never gets back more pages than it has
+          if (c < a.pool - to) a.free_pages[to + c] = row[c];     // a pool never gets back more pages than it has
       }
       const long long next = top + total;
       top = next > a.pool ? a.pool : (int)next;
-      __syncthreads();
     }
     __threadfence_block();
     __syncthreads();                                 // pages pushed are visible to the pops below
@@ -103,7 +102,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanA
 
   // ---- 2. - 3. lengths, grants, pages ----
   long long rows_before = 0, asked_before = 0, taken_before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += PLAN_THREADS) {
+  for (int b0 = 0; b0 < a.B; b0 += threads) {
     const int b = b0 + tid;
     int kv = 0, n = 0;
     if (b < a.B) {
@@ -113,55 +112,57 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanA
       n = n < 0 ? 0 : n;
     }
     long long total;
-    const long long rows_end = rows_before + block_scan(n, part, total);
+    const long long rows_end = rows_before + block_scan(n, part, waves, total);
     rows_before += total;
     const bool fits = b < a.B && (long long)kv + n <= cap && rows_end <= a.rows;
     const int held = pages_of(kv, a.shift);
     int need = fits ? pages_of(kv + n, a.shift) - held : 0;
-    const long long asked = asked_before + block_scan(need, part, total);
+    const long long asked = asked_before + block_scan(need, part, waves, total);
     asked_before += total;
     const bool granted = fits && (need == 0 || asked <= top);
     need = granted ? need : 0;
-    const long long taken = taken_before + block_scan(need, part, total);
+    const long long taken = taken_before + block_scan(need, part, waves, total);
     taken_before += total;
     const long long cu = rows_end - n;
-    s_kv[tid] = kv;
+    s_kv[tid] = granted ? kv : -1;
     s_cu[tid] = cu > 0x7fffffff ? 0x7fffffff : (int)cu;
-    s_need[tid] = granted ? need : -1;
-    s_take[tid] = (int)(taken - need);
     if (b < a.B) {
       a.cu_rows[b] = s_cu[tid];
       a.granted[b] = granted;
       a.kv_lens[b] = granted ? kv + n : kv;
     }
     if (b == a.B - 1) {
-      s_cu[tid + 1] = rows_end > 0x7fffffff ? 0x7fffffff : (int)rows_end;
-      a.cu_rows[a.B] = s_cu[tid + 1];
+      const int end = rows_end > 0x7fffffff ? 0x7fffffff : (int)rows_end;
+      s_cu[tid + 1] = end;
+      a.cu_rows[a.B] = end;
     }
-    __syncthreads();
-    const int rows = a.B - b0 < PLAN_THREADS ? a.B - b0 : PLAN_THREADS;
-    for (int i = wave; i < rows; i += PLAN_WAVES) {
-      int32_t* row = a.table + (size_t)(b0 + i) * a.table_row + pages_of(s_kv[i], a.shift);
-      const int from = top - 1 - s_take[i], count = s_need[i];
-      for (int c = lane; c < count; c += 64) row[c] = a.free_pages[from - c];
+    const int from = top - 1 - (int)(taken - need);
+    if (need > 0 && need <= OWN_PAGES) {
+      int32_t* row = a.table + (size_t)b * a.table_row + held;
+      for (int c = 0; c < need; ++c) row[c] = a.free_pages[from - c];
     }
-    __syncthreads();
+    for (unsigned long long m = __ballot(need > OWN_PAGES); m; m &= m - 1) {
+      const int i = __ffsll(m) - 1;
+      const int count = __shfl(need, i), f = __shfl(from, i);
+      int32_t* row = a.table + (size_t)(b - lane + i) * a.table_row + __shfl(held, i);
+      for (int c = lane; c < count; c += 64) row[c] = a.free_pages[f - c];
+    }
   }
   if (tid == 0) *a.free_count = top - (int)taken_before;
 
-  // ---- 4. slots of a short step (B <= PLAN_THREADS: the last trip's LDS arrays describe every request) ----
+  // ---- 4. slots of a short step (one trip of the loop above: the LDS arrays describe every request) ----
   if (!inline_slots) return;
   __threadfence_block();
   __syncthreads();
-  for (int i = tid; i < a.rows; i += PLAN_THREADS) {
+  for (int i = tid; i < a.rows; i += threads) {
     long long slot = -1;
     if (i < s_cu[a.B]) {
-      int lo = 0, hi = a.B;                          // the last request that starts at or before row i and is not empty
+      int lo = 0, hi = a.B;                          // the last request that starts at or before row i (it is not empty)
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (s_cu[mid] <= i) lo = mid; else hi = mid;
       }
-      if (s_need[lo] >= 0) slot = slot_of(a.table + (size_t)lo * a.table_row, s_kv[lo] + i - s_cu[lo], a.shift);
+      if (s_kv[lo] >= 0) slot = slot_of(a.table + (size_t)lo * a.table_row, s_kv[lo] + i - s_cu[lo], a.shift);
     }
     a.slots[i] = slot;
   }
@@ -220,7 +221,9 @@ int launch_page_plan(const PagePlanArgs& a, hipStream_t stream) {
   if (((long long)a.width << a.shift) > 0x7fffffffll) return fail("page_plan: a table of %d pages describes more than 2^31 - 1 tokens", a.width);
   if (!a.kv_lens || !a.new_lens || !a.table || !a.free_pages || !a.free_count || !a.cu_rows || !a.granted || (a.rows > 0 && !a.slots)) return fail("page_plan: null operand");
   const bool inl = a.B <= PLAN_THREADS && a.rows <= PLAN_INLINE_ROWS;
-  page_plan_kernel<<<1, PLAN_THREADS, 0, stream>>>(a, inl ? 1 : 0);
+  int threads = a.B > a.rows || !inl ? a.B : a.rows;
+  threads = threads > PLAN_THREADS ? PLAN_THREADS : (threads + 63) / 64 * 64;
+  page_plan_kernel<<<1, threads, 0, stream>>>(a, inl ? 1 : 0);
   if (!inl && a.rows > 0) page_slots_kernel<<<(a.rows - 1) / 256 + 1, 256, 0, stream>>>(a);
   return check_launch("page_plan");
 }
