@@ -6,15 +6,19 @@
 //   top-p : token i while the mass of those before it is below p times the mass that top-k left;    (p >= 1: all)
 //   min-p : tokens with w_i >= min_p                                 (w of the largest is 1)
 // The first token is always kept.  Over the kept ones in index order, with C_i the running sum of w and C the whole sum,
-// the token drawn for a given u in [0, 1) is the first with C_i > u C.  t <= 0 takes the largest logit.
+// the token drawn for a given u in [0, 1) is the first with C_i > u C.  t <= 0 takes the first maximum.
 //
 // A token is a comparison of a sum with a border, so sums must not depend on the order of their terms: weights are
-// formed in fp64 and rounded to integers in units of 2^-45 (the largest is 2^45; up to 2^18 of them stay below 2^63),
-// and integers add up exactly in any order, LDS atomics included.  A weight below 2^-46 of the largest counts as 0.
+// formed in fp64 and rounded to integers in units of 2^-b, b = min(51, 63 - ceil(log2 vocab)), so that no sum passes
+// 2^63, and integers add up exactly in any order, LDS atomics included.  A weight below half a unit counts as 0.
 //
-// One workgroup per row.  The head's last token is found by counting, not sorting: a histogram (counts and masses) over
-// 2048 equal steps of (max - x) / t gives the step it lies in, finer histograms over the values' bit patterns inside
-// that step give its value, and among equal values an index count gives the token.
+// One workgroup per row; a wave takes a contiguous piece of it.  The head's last token is found by counting, not
+// sorting: a histogram (counts or masses) over equal steps of (max - x) / t gives the step it lies in, histograms over
+// the bit patterns inside that step give its value, and a count over equal values gives the token.  Elements that the
+// first histogram leaves in question go to a list in LDS (in index order, a segment per wave): everything above the k-th when
+// top-k is on, so that the rest of the work runs on the list, or the one step that top-p ends in.  A list that does not
+// fit is not made, and the same code runs over the row again.
+#include <float.h>
 #include <math.h>
 
 #include "common.h"
@@ -24,454 +28,614 @@ namespace fcenc {
 
 namespace {
 
-constexpr int NBINS = 2048;
-constexpr float BINS_PER_UNIT = 64.f;             // 2048 steps reach down to exp(-32), below a weight's last bit
-constexpr int MAX_VOCAB = 1 << 18;
 constexpr int MAX_WAVES = 16;
-constexpr double UNIT = 35184372088832.0;         // 2^45
+constexpr int BINS_PER_WAVE = 128;                // two bins per thread
+constexpr int SEG = 512;                          // list entries per wave
+constexpr float RANGE = 32.f;                     // the first histogram reaches down to exp(-32), about where weights end
+constexpr int MAX_VOCAB = 1 << 18;
+constexpr int TABLE = 256;
+constexpr double MAGIC = 4503599627370496.0;      // 2^52: adding it leaves a rounded integer in the low 52 bits
 using u64 = unsigned long long;
 
-struct SampleLds {
-  u64 mass[NBINS];
-  u64 part_m[MAX_WAVES];
-  double table[32];                               // 2^(j / 32)
-  unsigned count[NBINS];
-  unsigned part_c[MAX_WAVES];
-  unsigned lo, hi;                                // range of keys
-  // a border found in the bins
-  u64 mass_before;
-  unsigned count_before;
-  int bin;
-  int token;
+// 2^(j / 256)
+struct ExpTable {
+  double v[TABLE];
+  constexpr ExpTable() : v() {
+    for (int j = 0; j < TABLE; ++j) {
+      const double x = j * (0.693147180559945309417 / TABLE);
+      double term = 1.0, sum = 1.0;
+      for (int i = 1; i < 24; ++i) {
+        term *= x / i;
+        sum += term;
+      }
+      v[j] = sum;
+    }
+  }
 };
+__device__ constexpr ExpTable exp_table{};
 
-// larger values have larger keys; -0 counts as 0, NaN as -inf
+struct SampleLds {
+  u64* mass;                 // [bins]
+  u64* part_m;               // [waves]
+  double* table;             // [TABLE]
+  unsigned* count;           // [bins]
+  unsigned* part_c;          // [waves]
+  unsigned* seg_n;           // [waves] list entries
+  float* seg_x;              // [waves][SEG]
+  int* seg_i;                // [waves][SEG]
+  unsigned* lo;              // range of keys: lo, hi
+  u64* found_m;              // a border found in the bins: mass before it,
+  unsigned* found;           //   bin, count before it; [2]: a token index
+};
+__host__ __device__ constexpr int lds_bytes(int waves) {
+  return waves * BINS_PER_WAVE * 12 + waves * (8 + 4 + 4) + TABLE * 8 + waves * SEG * 8 + 8 + 8 + 16;
+}
+
+__device__ __forceinline__ SampleLds carve(char* p, int waves) {
+  SampleLds l;
+  auto take = [&](int bytes) { char* at = p; p += bytes; return at; };
+  l.mass = reinterpret_cast<u64*>(take(waves * BINS_PER_WAVE * 8));
+  l.part_m = reinterpret_cast<u64*>(take(waves * 8));
+  l.table = reinterpret_cast<double*>(take(TABLE * 8));
+  l.found_m = reinterpret_cast<u64*>(take(8));
+  l.count = reinterpret_cast<unsigned*>(take(waves * BINS_PER_WAVE * 4));
+  l.part_c = reinterpret_cast<unsigned*>(take(waves * 4));
+  l.seg_n = reinterpret_cast<unsigned*>(take(waves * 4));
+  l.seg_x = reinterpret_cast<float*>(take(waves * SEG * 4));
+  l.seg_i = reinterpret_cast<int*>(take(waves * SEG * 4));
+  l.lo = reinterpret_cast<unsigned*>(take(8));
+  l.found = reinterpret_cast<unsigned*>(take(16));
+  return l;
+}
+
+// smaller values have larger keys; -0 counts as 0
 __device__ __forceinline__ unsigned key_of(float x) {
-  const unsigned u = __builtin_bit_cast(unsigned, x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const unsigned u = __builtin_bit_cast(unsigned, x == 0.f ? 0.f : x);
+  return u & 0x80000000u ? u : ~(u | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(unsigned key) {
-  return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key);
+  return __builtin_bit_cast(float, key & 0x80000000u ? key : ~key & 0x7fffffffu);
 }
-__device__ __forceinline__ float clean(float x) { return x == x ? (x == 0.f ? 0.f : x) : -INFINITY; }
+// NaN counts as -inf, +inf as the largest finite number
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 
-// eight logits from element e of the row on; elements behind the row are -inf
-__device__ __forceinline__ void load_logits(const float* row, int e, int n, float (&x)[8]) {
-  struct __attribute__((packed, aligned(4))) V { float v[8]; };
+struct Raw8F { f32x4 lo, hi; };
+__device__ __forceinline__ float raw_at(const Raw8F& r, int i) { return i < 4 ? r.lo[i] : r.hi[i - 4]; }
+__device__ __forceinline__ float raw_at(const u32x4& r, int i) {
+  return __builtin_bit_cast(float, i & 1 ? r[i >> 1] & 0xffff0000u : r[i >> 1] << 16);
+}
+// eight logits, at any alignment of the type
+__device__ __forceinline__ Raw8F load_whole(const float* p) {
+  struct __attribute__((packed, aligned(4))) V { f32x4 a, b; };
+  const V v = *reinterpret_cast<const V*>(p);
+  return Raw8F{v.a, v.b};
+}
+__device__ __forceinline__ u32x4 load_whole(const bf16* p) {
+  struct __attribute__((packed, aligned(2))) V { u32x4 a; };
+  return reinterpret_cast<const V*>(p)->a;
+}
+// the same from element e of the row on; -inf behind the row's end
+__device__ __forceinline__ Raw8F load_raw(const float* row, int e, int n) {
+  Raw8F r;
   if (e + 8 <= n) {
-    const V v = *reinterpret_cast<const V*>(row + e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = clean(v.v[i]);
+    r = load_whole(row + e);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = e + i < n ? clean(row[e + i]) : -INFINITY;
+    for (int i = 0; i < 8; ++i) {
+      const float x = e + i < n ? row[e + i] : -INFINITY;
+      if (i < 4) r.lo[i] = x; else r.hi[i - 4] = x;
+    }
   }
+  return r;
 }
-__device__ __forceinline__ void load_logits(const bf16* row, int e, int n, float (&x)[8]) {
-  struct __attribute__((packed, aligned(2))) V { bf16 v[8]; };
-  if (e + 8 <= n) {
-    const V v = *reinterpret_cast<const V*>(row + e);
+__device__ __forceinline__ u32x4 load_raw(const bf16* row, int e, int n) {
+  if (e + 8 <= n) return load_whole(row + e);
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+  u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = clean((float)v.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = e + i < n ? clean((float)row[e + i]) : -INFINITY;
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = e + 2 * i < n ? p[e + 2 * i] : 0xff80u, b = e + 2 * i + 1 < n ? p[e + 2 * i + 1] : 0xff80u;
+    r[i] = a | (b << 16);
   }
-}
-
-// exp of z <= 0 with z > -40, relative error below 1e-14: z = (32 n + j + f) ln 2 / 32, |f| <= 1/2, and the Taylor sum of
-// exp(f ln 2 / 32) to the fifth power leaves (0.0109)^6 / 720 = 2e-15
-__device__ __forceinline__ double exp_neg(double z, const double* table) {
-  const double s = z * (32.0 / M_LN2);
-  const double k = rint(s);
-  const double f = (s - k) * (M_LN2 / 32.0);
-  const int n = (int)k;
-  double p = fma(f, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(f, p, 1.0 / 6.0);
-  p = fma(f, p, 0.5);
-  p = fma(f, p, 1.0);
-  p = fma(f, p, 1.0);
-  return ldexp(p * table[n & 31], n >> 5);
+  return r;
 }
 
 struct RowParams {
   float top;                 // the largest logit
-  float bins;                // steps per unit of logit
-  double inv_t;
+  float bins;                // steps of the first histogram per unit of logit
+  int nbins;
+  double c;                  // 256 / (t ln 2)
 };
 
+// exp((x - top) / t) in weight units, not yet rounded: with s = 256 log2(...) = 256 n + j + f, |f| <= 1/2, it is 2^n table[j]
+// exp(f ln 2 / 256); the Taylor sum to the third power leaves (0.00136)^4 / 24 = 1.4e-13.
 __device__ __forceinline__ double weight(float x, const RowParams& p, const double* table) {
-  if (x == p.top) return 1.0;
-  const double z = ((double)x - (double)p.top) * p.inv_t;
-  return z > -33.0 ? exp_neg(z, table) : 0.0;
+  constexpr double L = 0.693147180559945309417 / TABLE;
+  const double s = fmax(((double)x - (double)p.top) * p.c, -40.0 / L);
+  const double k = s + 1.5 * MAGIC;                    // an integer in the low word
+  const int n = (int)(unsigned)__builtin_bit_cast(u64, k);
+  const double f = s - (k - 1.5 * MAGIC);
+  double q = fma(f, L * L * L / 6.0, L * L / 2.0);
+  q = fma(f, q, L);
+  q = fma(f, q, 1.0);
+  return ldexp(q * table[n & (TABLE - 1)], n >> 8);
 }
-__device__ __forceinline__ u64 units(double w) { return (u64)(w * UNIT + 0.5); }
+__device__ __forceinline__ u64 rounded(double w) { return __builtin_bit_cast(u64, w + MAGIC) & 0xfffffffffffffull; }
+__device__ __forceinline__ u64 units(float x, const RowParams& p, const double* table) { return rounded(weight(x, p, table)); }
 __device__ __forceinline__ int bin_of(float x, const RowParams& p) {
-  if (x == p.top) return 0;
-  const float d = (p.top - x) * p.bins;              // both steps round monotonically
-  return d < (float)(NBINS - 1) ? (int)d : NBINS - 1;
+  const float d = (p.top - x) * p.bins;                // both steps round monotonically
+  return d < (float)(p.nbins - 1) ? (int)d : p.nbins - 1;
 }
 
-__device__ __forceinline__ u64 wave_sum(u64 v) {
+template <typename V>
+__device__ __forceinline__ V wave_total(V v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
-
-// calls f(index, eight logits) for the vectors of [from, to) that belong to this wave: a contiguous piece per wave
-template <typename T, typename F>
-__device__ __forceinline__ void for_row(const T* row, int from, int to, int n, int wave, int waves, int lane, F f) {
-  const int vecs = (to - from + 7) >> 3;
-  const int per = ((vecs + waves - 1) / waves + 63) & ~63;      // whole wave instructions
-  const int end = (wave + 1) * per < vecs ? (wave + 1) * per : vecs;
-  for (int v = wave * per + lane; v < end; v += 64) {
-    float x[8];
-    load_logits(row, from + 8 * v, n, x);
-    f(from + 8 * v, x);
-  }
-}
-__device__ __forceinline__ int piece(int from, int to, int waves) {           // elements of a wave's piece
-  const int vecs = (to - from + 7) >> 3;
-  return (((vecs + waves - 1) / waves + 63) & ~63) * 8;
-}
-
-// The bin in which the running count reaches `k` (k > 0) or else the running mass reaches `target`, starting from
-// count0 / mass0 in front of bin 0: into lds.bin, .count_before, .mass_before.
-__device__ __forceinline__ void find_bin(SampleLds& lds, unsigned k, double target, unsigned count0, u64 mass0, int waves) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = NBINS / (64 * waves);
-  __syncthreads();
-  unsigned c = 0;
-  u64 m = 0;
-  for (int i = 0; i < per; ++i) {
-    c += lds.count[tid * per + i];
-    m += lds.mass[tid * per + i];
-  }
-  unsigned ci = c;
-  u64 mi = m;
+template <typename V>
+__device__ __forceinline__ V wave_running(V v, int lane) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const unsigned cu = __shfl_up(ci, o);
-    const u64 mu = __shfl_up(mi, o);
-    if (lane >= o) {
-      ci += cu;
-      mi += mu;
+    const V u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// ---- where the elements come from: the row in memory, or the list in LDS ----
+template <typename T>
+struct RowSource {
+  static constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2;         // vectors in flight per lane
+  const T* row;
+  int n, wave, waves, lane;
+
+  // f(index of the first, eight raw logits) for the vectors of [from, to) in this wave's piece of that range
+  template <typename F>
+  __device__ __forceinline__ void vectors(int from, int to, F f) const {
+    const int per = piece(from, to) >> 3, vecs = (to - from + 7) >> 3;
+    const int end = (wave + 1) * per < vecs ? (wave + 1) * per : vecs;
+    int v0 = wave * per;
+    for (; v0 + 64 * AHEAD <= end && from + 8 * (v0 + 64 * AHEAD) <= n; v0 += 64 * AHEAD) {
+      decltype(load_raw(row, 0, 0)) raw[AHEAD];
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) raw[a] = load_whole(row + from + 8 * (v0 + 64 * a + lane));
+#pragma unroll
+      for (int a = 0; a < AHEAD; ++a) f(from + 8 * (v0 + 64 * a + lane), raw[a]);
+    }
+    for (; v0 < end; v0 += 64) {                       // every lane takes part; those past the piece see nothing but -inf
+      const int e = v0 + lane < end ? from + 8 * (v0 + lane) : n;
+      f(e, load_raw(row, e, n));
     }
   }
+  // f(index, value) for the elements of that piece, and -inf at indices >= n that fill up the last wave instruction
+  template <typename F>
+  __device__ __forceinline__ void each(int from, int to, F f) const {
+    vectors(from, to, [&](int e, const auto& raw) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f(e + i, clean(raw_at(raw, i)));
+    });
+  }
+  template <typename F>
+  __device__ __forceinline__ void all(F f) const { each(0, n, f); }
+  // elements of a wave's piece: whole wave instructions
+  __device__ __forceinline__ int piece(int from, int to) const {
+    const int vecs = (to - from + 7) >> 3;
+    return (((vecs + waves - 1) / waves + 63) & ~63) * 8;
+  }
+};
+
+struct ListSource {
+  const SampleLds& lds;
+  int wave, waves, lane;
+  template <typename F>
+  __device__ __forceinline__ void all(F f) const {
+    const int n = (int)lds.seg_n[wave];
+    for (int i = lane; i < n; i += 64) f(lds.seg_i[wave * SEG + i], lds.seg_x[wave * SEG + i]);
+  }
+};
+
+// `locate` finds the first element, in index order, at which the running sum of g(index, value) exceeds target_of(total),
+// and gives its index to every thread.  The wave whose piece it lies in:
+template <typename F>
+__device__ __forceinline__ int pick_wave(const SampleLds& lds, u64 mine, int waves, int wave, int lane, u64& target, bool first,
+                                         F target_of) {
+  const u64 m = wave_total(mine);
+  __syncthreads();
+  if (lane == 0) lds.part_m[wave] = m;
+  __syncthreads();
+  if (first) {
+    u64 total = 0;
+    for (int w = 0; w < waves; ++w) total += lds.part_m[w];
+    target = target_of(total);
+  }
+  int w = 0;
+  u64 before = 0;
+  while (w < waves - 1 && before + lds.part_m[w] <= target) before += lds.part_m[w++];
+  target -= before;
+  return w;
+}
+// eight values per lane, in order: the position (lane and element) at which the running sum exceeds `target`, -1 if none
+__device__ __forceinline__ int pick_in_wave(const u64 (&v)[8], int lane, u64& target) {
+  u64 sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum += v[i];
+  const u64 incl = wave_running(sum, lane);
+  const u64 hit = __ballot(incl > target);
+  if (!hit) {
+    target -= __shfl(incl, 63);
+    return -1;
+  }
+  const int l = __ffsll(hit) - 1;
+  u64 run = incl - sum;
+  int at = 7;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    u64 upto = run;
+#pragma unroll
+    for (int j = 0; j <= i; ++j) upto += v[j];
+    if (upto > target) at = i;
+  }
+  return 8 * l + __shfl(at, l);
+}
+
+template <typename T, typename G, typename F>
+__device__ __forceinline__ int locate(const SampleLds& lds, const RowSource<T>& s, G g, F target_of) {
+  u64 target = 0;
+  int from = 0, to = s.n;
+  for (int level = 0; level < 2; ++level) {
+    u64 m = 0;
+    s.each(from, to, [&](int e, float x) { m += g(e, x); });
+    const int w = pick_wave(lds, m, s.waves, s.wave, s.lane, target, level == 0, target_of);
+    const int step = s.piece(from, to);
+    from += w * step;
+    to = from + step < to ? from + step : to;
+    if (s.waves == 1) break;
+  }
+  __syncthreads();
+  if (s.wave == 0) {                                           // 512 to 1024 elements
+    int at = -1;
+    for (int e0 = from; e0 < to && at < 0; e0 += 512) {
+      const auto raw = load_raw(s.row, e0 + 8 * s.lane < to ? e0 + 8 * s.lane : s.n, s.n);
+      u64 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int e = e0 + 8 * s.lane + i;
+        v[i] = e < to ? g(e, clean(raw_at(raw, i))) : 0;
+      }
+      at = pick_in_wave(v, s.lane, target);
+      if (at >= 0) at += e0;
+    }
+    if (s.lane == 0) lds.found[2] = (unsigned)at;
+  }
+  __syncthreads();
+  return (int)lds.found[2];
+}
+template <typename G, typename F>
+__device__ __forceinline__ int locate(const SampleLds& lds, const ListSource& s, G g, F target_of) {
+  u64 target = 0, m = 0;
+  s.all([&](int e, float x) { m += g(e, x); });
+  const int w = pick_wave(lds, m, s.waves, s.wave, s.lane, target, true, target_of);
+  __syncthreads();
+  if (s.wave == 0) {
+    static_assert(SEG == 512, "a segment is eight entries per lane");
+    const int n = (int)lds.seg_n[w];
+    u64 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = 8 * s.lane + i;
+      v[i] = k < n ? g(lds.seg_i[w * SEG + k], lds.seg_x[w * SEG + k]) : 0;
+    }
+    const int at = pick_in_wave(v, s.lane, target);
+    if (s.lane == 0) lds.found[2] = (unsigned)(at >= 0 && at < n ? lds.seg_i[w * SEG + at] : -1);
+  }
+  __syncthreads();
+  return (int)lds.found[2];
+}
+
+// Puts the elements that `want` names into the list; false (for every thread) if a segment does not hold its wave's share.
+template <typename T, typename W>
+__device__ __forceinline__ bool make_list(const SampleLds& lds, const RowSource<T>& s, W want) {
+  unsigned n = 0;
+  s.vectors(0, s.n, [&](int e, const auto& raw) {
+    unsigned mask = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (want(clean(raw_at(raw, i)))) mask |= 1u << i;
+    const int left = s.n - e;                                  // no index behind the row's end
+    if (left < 8) mask &= (1u << left) - 1;
+    if (!__any(mask != 0)) return;
+    const unsigned c = __popc(mask);
+    const unsigned incl = wave_running(c, s.lane);
+    unsigned at = n + incl - c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (mask >> i & 1) {
+        if (at < SEG) {
+          lds.seg_x[s.wave * SEG + at] = clean(raw_at(raw, i));
+          lds.seg_i[s.wave * SEG + at] = e + i;
+        }
+        ++at;
+      }
+    n = __builtin_amdgcn_readlane(n + incl, 63);
+  });
+  __syncthreads();
+  if (s.lane == 0) lds.seg_n[s.wave] = n;
+  __syncthreads();
+  bool fits = true;
+  for (int w = 0; w < s.waves; ++w) fits = fits && lds.seg_n[w] <= SEG;
+  return fits;
+}
+
+__device__ __forceinline__ void clear_bins(const SampleLds& lds) {
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    lds.count[i * blockDim.x + threadIdx.x] = 0;
+    lds.mass[i * blockDim.x + threadIdx.x] = 0;
+  }
+  __syncthreads();
+}
+
+struct Found {
+  int bin;
+  unsigned count;            // before the bin
+  u64 mass;
+};
+// The bin in which the running count reaches `k` (k > 0) or else the running mass reaches `target`, counting from `count0` /
+// `mass0` in front of bin 0.
+__device__ __forceinline__ Found find_bin(const SampleLds& lds, unsigned k, double target, unsigned count0, u64 mass0, int waves) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __syncthreads();
+  const unsigned c0 = lds.count[2 * tid], c1 = lds.count[2 * tid + 1];
+  const u64 m0 = lds.mass[2 * tid], m1 = lds.mass[2 * tid + 1];
+  const unsigned ci = wave_running(c0 + c1, lane);
+  const u64 mi = wave_running(m0 + m1, lane);
   if (lane == 63) {
     lds.part_c[wave] = ci;
     lds.part_m[wave] = mi;
   }
   __syncthreads();
-  unsigned cb = count0 + ci - c;
-  u64 mb = mass0 + mi - m;
+  unsigned cb = count0 + ci - (c0 + c1);
+  u64 mb = mass0 + mi - (m0 + m1);
   for (int w = 0; w < wave; ++w) {
     cb += lds.part_c[w];
     mb += lds.part_m[w];
   }
-  for (int i = 0; i < per; ++i) {
-    const unsigned cn = lds.count[tid * per + i];
-    const u64 mn = lds.mass[tid * per + i];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const unsigned cn = i ? c1 : c0;
+    const u64 mn = i ? m1 : m0;
     const bool here = k > 0 ? cb < k && k <= cb + cn : (double)mb < target && (double)(mb + mn) >= target;
     if (here) {
-      lds.bin = tid * per + i;
-      lds.count_before = cb;
-      lds.mass_before = mb;
+      lds.found[0] = (unsigned)(2 * tid + i);
+      lds.found[1] = cb;
+      *lds.found_m = mb;
     }
     cb += cn;
     mb += mn;
   }
   __syncthreads();
-}
-
-__device__ __forceinline__ void clear_bins(SampleLds& lds, int threads) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < NBINS; i += threads) {
-    lds.count[i] = 0;
-    lds.mass[i] = 0;
-  }
-  __syncthreads();
+  return Found{(int)lds.found[0], lds.found[1], *lds.found_m};
 }
 
 struct Border {              // the last kept token: its key, how many of the tokens with that key are kept, what lies before
   unsigned key, ties;
   u64 mass_before;
 };
-
-// Narrows the step `bin0` of the first histogram down to one value.
-template <typename T>
-__device__ __forceinline__ Border refine(SampleLds& lds, const T* row, int n, const RowParams& p, unsigned k, double target,
-                                         int waves) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int bin0 = lds.bin;
-  unsigned count0 = lds.count_before;
-  u64 mass0 = lds.mass_before;
+// Narrows step `at` of the first histogram down to one value; the source holds at least that step's elements.
+template <typename S>
+__device__ __forceinline__ Border refine(const SampleLds& lds, const S& s, const RowParams& p, unsigned k, double target, Found at) {
+  const int bin0 = at.bin;
   __syncthreads();
-  if (tid == 0) {
-    lds.lo = 0xffffffffu;
-    lds.hi = 0;
+  if (threadIdx.x == 0) {
+    lds.lo[0] = 0xffffffffu;
+    lds.lo[1] = 0;
   }
   __syncthreads();
-  unsigned klo = 0xffffffffu, khi = 0;                   // inverted keys: rising with falling value
-  for_row(row, 0, n, n, wave, waves, lane, [&](int e, const float(&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (e + i < n && bin_of(x[i], p) == bin0) {
-        const unsigned key = ~key_of(x[i]);
-        klo = key < klo ? key : klo;
-        khi = key > khi ? key : khi;
-      }
+  unsigned klo = 0xffffffffu, khi = 0;
+  s.all([&](int e, float x) {
+    if (bin_of(x, p) == bin0) {
+      const unsigned key = key_of(x);
+      klo = key < klo ? key : klo;
+      khi = key > khi ? key : khi;
+    }
   });
   if (klo <= khi) {
-    atomicMin(&lds.lo, klo);
-    atomicMax(&lds.hi, khi);
+    atomicMin(&lds.lo[0], klo);
+    atomicMax(&lds.lo[1], khi);
   }
   __syncthreads();
-  unsigned base = lds.lo, top = lds.hi;
+  unsigned base = lds.lo[0], top = lds.lo[1];
+  const int log_bins = 31 - __clz(p.nbins);
   while (top != base) {
     const int bits = 32 - __clz((int)(top - base));
-    const int shift = bits > 11 ? bits - 11 : 0;
-    clear_bins(lds, 64 * waves);
-    for_row(row, 0, n, n, wave, waves, lane, [&](int e, const float(&x)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const unsigned key = ~key_of(x[i]);
-        if (e + i < n && key >= base && key <= top) {
-          atomicAdd(&lds.count[(key - base) >> shift], 1u);
-          atomicAdd(&lds.mass[(key - base) >> shift], units(weight(x[i], p, lds.table)));
-        }
+    const int shift = bits > log_bins ? bits - log_bins : 0;
+    clear_bins(lds);
+    s.all([&](int e, float x) {
+      const unsigned key = key_of(x);
+      if (key >= base && key <= top) {
+        atomicAdd(&lds.count[(key - base) >> shift], 1u);
+        atomicAdd(&lds.mass[(key - base) >> shift], units(x, p, lds.table));
       }
     });
-    find_bin(lds, k, target, count0, mass0, waves);
-    count0 = lds.count_before;
-    mass0 = lds.mass_before;
-    base += (unsigned)lds.bin << shift;
+    at = find_bin(lds, k, target, at.count, at.mass, s.waves);
+    base += (unsigned)at.bin << shift;
     const unsigned end = base + ((1u << shift) - 1);
     top = end < top ? end : top;
   }
   Border b;
   b.key = base;
-  b.mass_before = mass0;
+  b.mass_before = at.mass;
   if (k > 0) {
-    b.ties = k - count0;
+    b.ties = k - at.count;
   } else {
-    const double w = (double)units(weight(value_of(~base), p, lds.table));
-    const double r = ceil((target - (double)mass0) / w);       // kept while mass0 + i w < target
+    const double r = ceil((target - (double)at.mass) / (double)units(value_of(base), p, lds.table));   // kept while mass + i w < target
     b.ties = r < 1.0 ? 1u : (r > (double)MAX_VOCAB ? (unsigned)MAX_VOCAB : (unsigned)r);
   }
   return b;
 }
 
+struct Limit {               // the tokens that are kept: values above x, and those equal to it up to an index
+  float x;
+  int index;
+};
+
+template <typename S>
+__device__ __forceinline__ int draw(const SampleLds& lds, const S& s, const RowParams& p, Limit lim, float min_p, float u) {
+  if (min_p > 0.f) {                                           // w >= min_p in terms of x, rounded up to a float
+    const double least = (double)p.top + log((double)fminf(min_p, 1.f)) * (TABLE / 0.693147180559945309417) / p.c;
+    float x = (float)least;
+    if ((double)x < least) x = nextafterf(x, INFINITY);
+    x = fminf(x, p.top);
+    if (x > lim.x) lim = Limit{x, 0x7fffffff};
+  }
+  if (!(u > 0.f))            // u = 0 (or NaN): the first kept token whose weight is a number at all, however small
+    return locate(lds, s, [&](int e, float x) -> u64 {
+      const bool kept = x > lim.x || (x == lim.x && e <= lim.index);
+      return kept && ((double)x - (double)p.top) * p.c > -745.13 * (TABLE / 0.693147180559945309417);
+    }, [](u64) -> u64 { return 0; });
+  u = u < 1.f ? u : 0.99999994f;
+  return locate(lds, s, [&](int e, float x) -> u64 {
+    const u64 w = units(x, p, lds.table);
+    return x > lim.x || (x == lim.x && e <= lim.index) ? w : 0;
+  }, [&](u64 total) -> u64 {
+    const u64 t = (u64)((double)u * (double)total);
+    return t < total ? t : total - 1;
+  });
+}
+template <typename S>
+__device__ __forceinline__ int tie_index(const SampleLds& lds, const S& s, float value, unsigned ties) {
+  return locate(lds, s, [&](int e, float x) -> u64 { return x == value; },
+                [&](u64 total) -> u64 { return (ties < total ? ties : total) - 1; });
+}
+
+// the mass histogram of the elements above `floor`, and its total
+template <typename S>
+__device__ __forceinline__ u64 mass_bins(const SampleLds& lds, const S& s, const RowParams& p, float floor) {
+  clear_bins(lds);
+  u64 m = 0;
+  s.all([&](int e, float x) {
+    u64 w = units(x, p, lds.table);
+    w = x > floor ? w : 0;
+    m += w;
+    atomicAdd(&lds.mass[w ? bin_of(x, p) : s.lane], w);        // no branch; nothing is added to some bin rather than to the last one
+  });
+  m = wave_total(m);
+  if (s.lane == 0) lds.part_m[s.wave] = m;
+  __syncthreads();
+  u64 total = 0;
+  for (int w = 0; w < s.waves; ++w) total += lds.part_m[w];
+  __syncthreads();
+  return total;
+}
+
+// top-k on, its step of the first histogram known: the rest of the row's work
+template <typename S>
+__device__ __forceinline__ int by_rank(const SampleLds& lds, const S& s, const RowParams& p, unsigned k, float top_p, float min_p,
+                                       float u, Found at) {
+  const Border b = refine(lds, s, p, k, 0.0, at);
+  float value = value_of(b.key);
+  unsigned ties = b.ties;
+  if (top_p < 1.f) {
+    // masses before the border's own value, then `ties` times that value's
+    const u64 before = mass_bins(lds, s, p, value);
+    const u64 w = units(value, p, lds.table);
+    const double target = (double)top_p * (double)(before + ties * w);
+    if ((double)before >= target) {
+      const Found f = find_bin(lds, 0, target, 0, 0, s.waves);
+      const Border c = refine(lds, s, p, 0, target, f);
+      value = value_of(c.key);
+      ties = c.ties;
+    } else {
+      const double r = ceil((target - (double)before) / (double)w);
+      ties = r < (double)ties ? (r < 1.0 ? 1u : (unsigned)r) : ties;
+    }
+  }
+  return draw(lds, s, p, Limit{value, tie_index(lds, s, value, ties)}, min_p, u);
+}
+
 template <typename T>
 __global__ __launch_bounds__(64 * MAX_WAVES) void sample_kernel(const SampleArgs a) {
-  __shared__ SampleLds lds;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = blockDim.x, waves = threads >> 6;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const SampleLds lds = carve(smem, waves);
   const int r = blockIdx.x, n = a.vocab;
-  const T* row = reinterpret_cast<const T*>(a.logits) + (long long)r * a.row_stride;
-  if (tid < 32) lds.table[tid] = exp2(tid / 32.0);
+  const RowSource<T> s{reinterpret_cast<const T*>(a.logits) + (long long)r * a.row_stride, n, wave, waves, lane};
+  const int log_n = n > 1 ? 32 - __clz(n - 1) : 0;
+  const double unit = ldexp(1.0, log_n > 12 ? 63 - log_n : 51);
+  for (int i = tid; i < TABLE; i += blockDim.x) lds.table[i] = exp_table.v[i] * unit;
 
-  // ---- the first of the largest ----
-  u64 best = 0;                                            // key, then the smaller index
-  for_row(row, 0, n, n, wave, waves, lane, [&](int e, const float(&x)[8]) {
+  // the largest logit, and the lane's first vector that holds its own largest
+  float top = -INFINITY;
+  int top_at = 0;
+  s.vectors(0, n, [&](int e, const auto& raw) {
+    float m = clean(raw_at(raw, 0));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const u64 c = ((u64)key_of(x[i]) << 32) | (unsigned)~(e + i);
-      best = e + i < n && c > best ? c : best;
-    }
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, clean(raw_at(raw, i)));
+    top_at = m > top ? e : top_at;
+    top = fmaxf(top, m);
   });
+  const float lane_top = top;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const u64 c = __shfl_xor(best, o);
-    best = c > best ? c : best;
-  }
-  if (lane == 0) lds.part_m[wave] = best;
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) lds.part_c[wave] = __builtin_bit_cast(unsigned, top);
   __syncthreads();
-  for (int w = 0; w < waves; ++w) best = lds.part_m[w] > best ? lds.part_m[w] : best;
-  RowParams p;
-  p.top = value_of((unsigned)(best >> 32));
+  for (int w = 0; w < waves; ++w) top = fmaxf(top, __builtin_bit_cast(float, lds.part_c[w]));
+  __syncthreads();
+
   const float t = a.temperature ? a.temperature[r] : 1.f;
   const int top_k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.f;
   const float min_p = a.min_p ? a.min_p[r] : 0.f;
-  if (p.top == -INFINITY || !(t > 0.f) || top_k == 1 || top_p <= 0.f) {
-    if (tid == 0) a.tokens[r] = p.top == -INFINITY ? -1 : (int)~(unsigned)best;
-    return;
-  }
-  p.bins = BINS_PER_UNIT / t;
-  p.inv_t = 1.0 / (double)t;
-
-  // ---- the last token that top-k and top-p keep ----
-  const bool by_k = top_k > 0 && top_k < n, by_p = top_p < 1.f;
-  unsigned last_key = 0xffffffffu, last_ties = 0xffffffffu;      // everything
-  if (by_k || by_p) {
-    clear_bins(lds, threads);
-    for_row(row, 0, n, n, wave, waves, lane, [&](int e, const float(&x)[8]) {
+  int token;
+  if (top == -INFINITY) {
+    token = -1;
+  } else if (!(t > 0.f) || top_k == 1 || top_p <= 0.f) {
+    if (tid == 0) lds.lo[0] = 0xffffffffu;
+    __syncthreads();
+    if (lane_top == top) atomicMin(&lds.lo[0], (unsigned)top_at);
+    __syncthreads();
+    const int e = (int)lds.lo[0];
+    const auto raw = load_raw(s.row, e, n);
+    token = e;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (e + i < n) {
-          const int bin = bin_of(x[i], p);
-          if (by_k) atomicAdd(&lds.count[bin], 1u);
-          if (by_p) atomicAdd(&lds.mass[bin], units(weight(x[i], p, lds.table)));
+    for (int i = 7; i >= 0; --i) token = clean(raw_at(raw, i)) == top ? e + i : token;
+  } else {
+    RowParams p;
+    p.top = top;
+    p.nbins = waves * BINS_PER_WAVE;
+    p.bins = fminf((float)p.nbins / RANGE / t, 1e30f);         // finite, so that the largest logit lies in bin 0
+    p.c = TABLE / 0.693147180559945309417 / (double)t;
+    const float u = a.u[r];
+    if (top_k > 0 && top_k < n) {
+      clear_bins(lds);
+      s.all([&](int e, float x) { atomicAdd(&lds.count[bin_of(x, p)], 1u); });
+      const Found at = find_bin(lds, (unsigned)top_k, 0.0, 0, 0, waves);
+      if (make_list(lds, s, [&](float x) { return bin_of(x, p) <= at.bin; }))
+        token = by_rank(lds, ListSource{lds, wave, waves, lane}, p, (unsigned)top_k, top_p, min_p, u, at);
+      else
+        token = by_rank(lds, s, p, (unsigned)top_k, top_p, min_p, u, at);
+    } else {
+      Limit lim{-INFINITY, n};
+      if (top_p < 1.f) {
+        const double target = (double)top_p * (double)mass_bins(lds, s, p, -INFINITY);
+        const Found at = find_bin(lds, 0, target, 0, 0, waves);
+        if (make_list(lds, s, [&](float x) { return bin_of(x, p) == at.bin; })) {
+          const ListSource l{lds, wave, waves, lane};
+          const Border b = refine(lds, l, p, 0, target, at);
+          lim.x = value_of(b.key);
+          lim.index = tie_index(lds, l, lim.x, b.ties);
+        } else {
+          const Border b = refine(lds, s, p, 0, target, at);
+          lim.x = value_of(b.key);
+          lim.index = tie_index(lds, s, lim.x, b.ties);
         }
-    });
-    __syncthreads();
-    u64 total = 0;
-    if (by_p) {
-      u64 m = 0;
-      for (int i = tid; i < NBINS; i += threads) m += lds.mass[i];
-      m = wave_sum(m);
-      if (lane == 0) lds.part_m[wave] = m;
-      __syncthreads();
-      for (int w = 0; w < waves; ++w) total += lds.part_m[w];
-      __syncthreads();
-    }
-    if (by_k) {
-      find_bin(lds, (unsigned)top_k, 0.0, 0, 0, waves);
-      const Border b = refine(lds, row, n, p, (unsigned)top_k, 0.0, waves);
-      last_key = b.key;
-      last_ties = b.ties;
-      if (by_p) {
-        total = b.mass_before + b.ties * units(weight(value_of(~b.key), p, lds.table));
-        clear_bins(lds, threads);
-        for_row(row, 0, n, n, wave, waves, lane, [&](int e, const float(&x)[8]) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (e + i < n && ~key_of(x[i]) <= last_key) atomicAdd(&lds.mass[bin_of(x[i], p)], units(weight(x[i], p, lds.table)));
-        });
-        __syncthreads();
       }
-    }
-    if (by_p) {
-      const double target = (double)top_p * (double)total;
-      find_bin(lds, 0, target, 0, 0, waves);
-      const Border b = refine(lds, row, n, p, 0, target, waves);
-      if (b.key < last_key) {
-        last_key = b.key;
-        last_ties = b.ties;
-      } else if (b.ties < last_ties) {
-        last_ties = b.ties;
-      }
+      token = draw(lds, s, p, lim, min_p, u);
     }
   }
-
-  // ---- among equal values the smaller indices: the last index kept ----
-  int last_index = n;
-  if (last_ties != 0xffffffffu) {
-    int from = 0, to = n;
-    unsigned want = last_ties;
-    for (int level = 0; level < 3 && to - from > 0; ++level) {    // 1/waves of the range per level, then one wave alone
-      unsigned c = 0;
-      for_row(row, from, to, n, wave, waves, lane, [&](int e, const float(&x)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c += e + i < to && ~key_of(x[i]) == last_key;
-      });
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
-      __syncthreads();
-      if (lane == 0) lds.part_c[wave] = c;
-      __syncthreads();
-      const int step = piece(from, to, waves);
-      int w = 0;
-      unsigned before = 0;
-      while (w < waves && before + lds.part_c[w] < want) before += lds.part_c[w++];
-      if (w == waves) {                                            // fewer than asked for: all of them are kept
-        from = to;
-        break;
-      }
-      want -= before;
-      const int f = from + w * step;
-      to = f + step < to ? f + step : to;
-      from = f;
-      __syncthreads();
-    }
-    if (from < to) {
-      if (wave == 0) {
-        int found = n;
-        for (int e0 = from; e0 < to; e0 += 64) {                   // 512 to 1024 elements at most
-          const int e = e0 + lane;
-          float x = -INFINITY;
-          if (e < to) x = clean((float)row[e]);
-          const u64 hit = __ballot(e < to && ~key_of(x) == last_key);
-          const unsigned c = (unsigned)__popcll(hit);
-          if (c >= want) {
-            u64 h = hit;
-            for (unsigned i = 1; i < want; ++i) h &= h - 1;
-            found = e0 + __ffsll(h) - 1;
-            break;
-          }
-          want -= c;
-        }
-        if (lane == 0) lds.token = found;
-      }
-      __syncthreads();
-      last_index = lds.token;
-      __syncthreads();
-    }
-  }
-
-  // ---- the draw ----
-  auto kept = [&](int e, float x, u64& m) {
-    const unsigned key = ~key_of(x);
-    m = 0;
-    if (key < last_key || (key == last_key && e <= last_index)) {
-      const double w = weight(x, p, lds.table);
-      if (w >= (double)min_p || x == p.top) m = units(w);
-    }
-  };
-  float u = a.u[r];
-  u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;                 // NaN draws as 0
-  int from = 0, to = n;
-  u64 target = 0;
-  for (int level = 0; level < 2; ++level) {
-    u64 m = 0;
-    for_row(row, from, to, n, wave, waves, lane, [&](int e, const float(&x)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        u64 v;
-        kept(e + i, x[i], v);
-        m += e + i < to ? v : 0;
-      }
-    });
-    m = wave_sum(m);
-    __syncthreads();
-    if (lane == 0) lds.part_m[wave] = m;
-    __syncthreads();
-    if (level == 0) {
-      u64 c = 0;
-      for (int w = 0; w < waves; ++w) c += lds.part_m[w];
-      target = (u64)((double)u * (double)c);
-      target = target < c ? target : c - 1;
-    }
-    const int step = piece(from, to, waves);
-    int w = 0;
-    u64 before = 0;
-    while (w < waves - 1 && before + lds.part_m[w] <= target) before += lds.part_m[w++];
-    target -= before;
-    const int f = from + w * step;
-    to = f + step < to ? f + step : to;
-    from = f;
-  }
-  if (wave == 0) {
-    int token = -1;
-    for (int e0 = from; e0 < to; e0 += 64) {
-      const int e = e0 + lane;
-      u64 v = 0;
-      if (e < to) kept(e, clean((float)row[e]), v);
-      u64 incl = v;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const u64 up = __shfl_up(incl, o);
-        if (lane >= o) incl += up;
-      }
-      const u64 hit = __ballot(incl > target);
-      if (hit) {
-        token = e0 + __ffsll(hit) - 1;
-        break;
-      }
-      target -= __shfl(incl, 63);
-    }
-    if (lane == 0) a.tokens[r] = token;
-  }
+  if (tid == 0) a.tokens[r] = token;
 }
 
 }  // namespace
@@ -483,11 +647,12 @@ int launch_sample_tokens(int dtype, const SampleArgs& a, hipStream_t stream) {
   if (a.rows > 1 && a.row_stride < a.vocab) return fail("sample_tokens: rows of %d logits overlap (stride %lld)", a.vocab, a.row_stride);
   if (!a.logits || !a.u || !a.tokens) return fail("sample_tokens: null operand");
   if ((uintptr_t)a.logits % (dtype == DT_BF16 ? 2 : 4)) return fail("sample_tokens: logits are not aligned to their type");
-  // a wave takes 512 logits at a time: as many waves as have some, in powers of two (the bins divide among them)
+  // a wave takes 512 logits at a time: as many waves as have some, in powers of two (the histogram has 128 bins per wave)
   int waves = 1;
   while (waves < MAX_WAVES && waves * 512 < a.vocab) waves *= 2;
-  if (dtype == DT_BF16) sample_kernel<bf16><<<a.rows, 64 * waves, 0, stream>>>(a);
-  else sample_kernel<float><<<a.rows, 64 * waves, 0, stream>>>(a);
+  auto k = dtype == DT_BF16 ? sample_kernel<bf16> : sample_kernel<float>;
+  if (reserve_lds(reinterpret_cast<const void*>(k), lds_bytes(MAX_WAVES)) != hipSuccess) return fail("sample_tokens: cannot reserve %d bytes of LDS", lds_bytes(MAX_WAVES));
+  k<<<a.rows, 64 * waves, lds_bytes(waves), stream>>>(a);
   return check_launch("sample_tokens");
 }
 
