@@ -31,17 +31,20 @@ namespace fcenc {
 
 namespace {
 
-constexpr uint32_t OOB = 0xF0000000u;       // an offset outside every descriptor
-constexpr int MAX_SPLITS = 64;
+constexpr uint32_t OOB = 0xE0000000u;       // an offset outside every descriptor, 16 slots of 2^24 bytes further on as well
+constexpr int MAX_SPLITS = 256;
 constexpr int STEP_WAVES = 4;
 constexpr int STEP_ROWS = 16;
 constexpr int CHUNK_ROWS = 128;             // rows of a tile of the chunk kernel
 constexpr int CHUNK_MIN = 32;               // requests with more rows (times heads per kv head) than this are its share
 
-// How a launch divides the work: `pieces` of the key axis here, `ws_pieces` in the workspace; `share` 0: every request,
-// 1: those of up to CHUNK_MIN rows and the rows behind the last request, 2: the longer ones.
+// How a launch divides the work.  `share` 0: every request; 1: those of up to CHUNK_MIN rows, `per_request` > 0 rows of
+// the chunk at most; 2: the longer ones and the rows behind the last request.
 struct Split {
-  int gc = 1, hchunks = 1, tt = 1, pieces = 1, ws_pieces = 1, share = 0;
+  int gc = 1, hchunks = 1, tt = 1, share = 0, per_request = 0;
+  int pieces = 1;                            // of the key axis; > 1: partial results go to the workspace from float `ws` on
+  long long ws = 0;
+  long long ws_rows = 0;                     // (row, head) pairs there: all of them, or per_request rows of every request
 };
 
 // Partial results of a split key axis: (m, l) of every (row, head, piece), then the unnormalised sums.
@@ -54,13 +57,26 @@ struct TileInfo {
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int clamp_rows(int v, int rows) { return v < 0 ? 0 : (v > rows ? rows : v); }
 
-// false: no such tile
-__device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, int tt, TileInfo& ti) {
+// false: no such tile, or not of this launch's share
+__device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const Split& sp, TileInfo& ti) {
+  const int tt = sp.tt;
   int lo = 0, hi = a.B + 1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    const int start = clamp_rows(uniform(a.cu_rows[mid]), a.rows) / tt + mid;
-    if (start <= tile) lo = mid; else hi = mid;
+  if (sp.share == 1) {                         // as many tiles for every request
+    const int each = (sp.per_request + tt - 1) / tt;
+    lo = tile / each;
+    tile = tile - lo * each + clamp_rows(uniform(a.cu_rows[lo]), a.rows) / tt + lo;
+  } else {
+    // 64 candidates at a time: one memory latency for up to 64 requests, two for up to 4096
+    const int lane = threadIdx.x & 63;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) >> 6;
+      const int b = lo + lane * step;
+      const bool at_or_before = b < hi && clamp_rows(a.cu_rows[b], a.rows) / tt + b <= tile;
+      const int k = __popcll(__ballot(at_or_before)) - 1;     // starts rise with b
+      lo = lo + (k > 0 ? k : 0) * step;
+      hi = hi < lo + step ? hi : lo + step;
+    }
+    lo = uniform(lo);
   }
   ti.b = lo;
   ti.c0 = clamp_rows(uniform(a.cu_rows[lo]), a.rows);
@@ -69,6 +85,8 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, int t
   ti.t0 = (tile - (ti.c0 / tt + lo)) * tt;
   ti.kv = 0;
   if (ti.t0 < 0 || ti.t0 >= ti.n) return false;
+  if (sp.share == 1 && ti.n > sp.per_request) return false;
+  if (sp.share == 2 && lo < a.B && ti.n <= sp.per_request) return false;
   if (lo < a.B) {
     const int cap = a.width << a.shift, kv = uniform(a.kv_lens[lo]);
     ti.kv = kv < 0 ? 0 : (kv > cap ? cap : kv);
@@ -76,8 +94,9 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, int t
   return true;
 }
 
-__device__ __forceinline__ bool is_chunk(const PageAttnArgs& a, const TileInfo& ti, int group) {
-  return ti.b < a.B && (long long)ti.n * group > CHUNK_MIN;
+// where the partial results of a (row of request b, head) lie
+__device__ __forceinline__ long long ws_row(const PageAttnArgs& a, const Split& sp, const TileInfo& ti, int row, int head) {
+  return (sp.share == 1 ? (long long)ti.b * sp.per_request + row : (long long)ti.c0 + row) * a.heads + head;
 }
 
 // V^T fragment of a [32 tokens][DP] tile in LDS: element j of lane (g, r) is V[token 16 (j >> 2) + 4 g + (j & 3)][dim 16 db + r]
@@ -169,8 +188,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   const int group = a.heads / a.kv_heads;
 
   TileInfo ti;
-  if (!find_tile(a, blockIdx.x, tt, ti)) return;
-  if (sp.share == 1 && is_chunk(a, ti, group)) return;
+  if (!find_tile(a, blockIdx.x, sp, ti)) return;
   const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
   const int last = first + (ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt) - 1;
   int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
@@ -215,6 +233,14 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   u32x4 vr[2][NV];
   bool page_ok[2];
   auto block_of = [&](int i) { return i < sb ? i : lob + i - sb; };
+  // of the block to fetch next, so that its loads need not wait for the table; left in vector registers until then (made
+  // uniform here, the wait for them would also wait for the K and V loads in front of them)
+  int pages[2];
+  auto find_pages = [&](int i) {
+    const int j0 = block_of(i) * 32;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) pages[t] = i < i1 && j0 + 16 * t < hi ? trow[(j0 + 16 * t) >> a.shift] : -1;
+  };
   // descriptors of the 16 tokens from tok0 on: bytes up to the last one that the tile sees
   auto fetch = [&](int i) {
     const int j0 = block_of(i) * 32;
@@ -223,33 +249,34 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
       const int tok0 = j0 + 16 * t;
       int left = hi - tok0;
       left = left > 16 ? 16 : left;
-      int page = -1;
-      if (left > 0) page = uniform(trow[tok0 >> a.shift]);
-      const bool ok = page >= 0 && page < a.n_pages;
-      page_ok[t] = ok || left <= 0;
+      const int page = uniform(pages[t]);
+      const bool ok = (page >= 0) & (page < a.n_pages) & (left > 0);
+      page_ok[t] = ok | (left <= 0);
       const int slot0 = tok0 & ((1 << a.shift) - 1);
       const char* kp = kbase + (long long)(ok ? page : 0) * a.k_page + (long long)slot0 * a.k_slot;
       const char* vp = vbase + (long long)(ok ? page : 0) * a.v_page + (long long)slot0 * a.v_slot;
       const __amdgpu_buffer_rsrc_t kd = buffer_of(kp, ok ? (left - 1) * a.k_slot + a.dim * ES : 0);
       const __amdgpu_buffer_rsrc_t vd = buffer_of(vp, ok ? (left - 1) * a.v_slot + a.dim * ES : 0);
       // tokens in front of the window and behind the sinks are seen by no row of the tile
-      const bool dead_k = tok0 + r < lo && tok0 + r >= sinks;
+      const bool dead_k = (tok0 + r < lo) & (tok0 + r >= sinks);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int d0 = 32 * ks + 8 * g;
-        kf[t][ks] = load_frag(kd, dead_k || d0 >= a.dim ? OOB : (uint32_t)(r * a.k_slot + d0 * ES), T{});
+        kf[t][ks] = load_frag(kd, (dead_k | (d0 >= a.dim)) ? OOB : (uint32_t)(r * a.k_slot + d0 * ES), T{});
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int row = lane / CPR + v * RPI, ch = lane % CPR;
-        const bool dead_v = tok0 + row < lo && tok0 + row >= sinks;
-        vr[t][v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(dead_v || ch * 16 >= a.dim * ES ? OOB : (uint32_t)(row * a.v_slot + ch * 16)), 0, 0);
+        const bool dead_v = (tok0 + row < lo) & (tok0 + row >= sinks);
+        vr[t][v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)((dead_v | (ch * 16 >= a.dim * ES)) ? OOB : (uint32_t)(row * a.v_slot + ch * 16)), 0, 0);
       }
     }
   };
 
   int i = i0 + wave;
+  find_pages(i);
   if (i < i1) fetch(i);
+  find_pages(i + STEP_WAVES);
   for (; i < i1; i += STEP_WAVES) {
     const int j0 = block_of(i) * 32;
     const bool ok0 = page_ok[0], ok1 = page_ok[1];
@@ -270,7 +297,10 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
         *reinterpret_cast<u32x4*>(vt + tile_off<ROWB>(16 * t + lane / CPR + v * RPI, lane % CPR)) = vr[t][v];
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-    if (i + STEP_WAVES < i1) fetch(i + STEP_WAVES);
+    if (i + STEP_WAVES < i1) {
+      fetch(i + STEP_WAVES);
+      find_pages(i + 2 * STEP_WAVES);
+    }
 
     bool inside = ok0 && ok1 && j0 + 31 <= (a.causal ? first : ti.kv - 1);
     if (a.window > 0) inside = inside && (j0 >= last - a.window + 1 || j0 + 31 < sinks);
@@ -341,24 +371,19 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
     for (int d = 0; d < DPT; ++d) acc[d] += src[d] * f;
   }
   const long long orow = (long long)(ti.c0 + ti.t0 + ort) * a.heads + kvh * group + orh;
-  if (sp.ws_pieces == 1) {
+  if (sp.pieces == 1) {
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);       // NaN stays NaN
     T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
 #pragma unroll
     for (int d = 0; d < DPT; ++d)
       if (d0 + d < a.dim) store_row(o + d0 + d, acc[d] * inv);
   } else {
-    const long long rows = (long long)a.rows * a.heads;
-    float* o = a.ws + ws_sums(rows, sp.ws_pieces) + (orow * sp.ws_pieces + split) * a.dim;
+    const long long at = ws_row(a, sp, ti, ti.t0 + ort, kvh * group + orh) * sp.pieces + split;
+    float* o = a.ws + sp.ws + ws_sums(sp.ws_rows, sp.pieces) + at * a.dim;
 #pragma unroll
     for (int d = 0; d < DPT; ++d)
       if (d0 + d < a.dim) o[d0 + d] = acc[d];
-    if ((tid & 15) == 0) {
-      float2* out = reinterpret_cast<float2*>(a.ws) + orow * sp.ws_pieces;
-      out[split] = float2{m, l};
-      if (split == 0)
-        for (int i = sp.pieces; i < sp.ws_pieces; ++i) out[i] = float2{-INFINITY, 0.f};
-    }
+    if ((tid & 15) == 0) reinterpret_cast<float2*>(a.ws + sp.ws)[at] = float2{m, l};
   }
 }
 
@@ -389,57 +414,67 @@ struct ChunkTile {
   static constexpr int KT = 64;                                  // tokens of a tile
   static constexpr int V_OFF = KT * ROWB;
   static constexpr int OK_OFF = 2 * KT * ROWB;                   // 4 flags: the page of every 16 tokens exists
-  static constexpr int STAGE = OK_OFF + 16;
+  static constexpr int STAGE = OK_OFF + 256;                     // keeps 256-byte rows aligned: see lds_at
   static constexpr int NST = sizeof(T) == 2 ? 2 : 1;             // fp32 tiles are twice as large: one stage, two barriers
   static constexpr int BYTES = NST * STAGE;
 };
 
-// K: 8 lanes that read one chunk of 8 rows hit 8 different ones.  V: the 4 rows x 32 bytes of a transposing read lie in
-// 128 different bytes.
+// Where 16-byte piece `ch` of row `row` lies, so that reads spread over the 256 bytes of the 64 LDS banks.  K: 16 rows that are
+// read at one piece hit 16 different ones.  V: a transposing read takes 4 rows x 32 bytes per 16 lanes, 64 bytes per 32
+// lanes, rows 4 apart in the wave's other half.
 template <int ROWB>
-__device__ __forceinline__ uint32_t k_off(int row, int ch) { return (uint32_t)(row * ROWB + ((ch ^ (row & 7)) << 4)); }
+__device__ __forceinline__ uint32_t k_off(int row, int ch) {
+  return (uint32_t)(row * ROWB + ((ch ^ (ROWB >= 256 ? row & 15 : (row >> 1) & 7)) << 4));
+}
 template <int ROWB>
 __device__ __forceinline__ uint32_t v_off(int row, int ch, bf16) {
-  return (uint32_t)(row * ROWB + ((ch ^ ((row & (ROWB >= 256 ? 7 : 3)) << 1)) << 4));
+  const int x = ROWB >= 256 ? (row & 3) << 2 : (row & 2) << 1;
+  return (uint32_t)(row * ROWB + ((ch ^ (x | (row >> 1 & 2))) << 4));
 }
 template <int ROWB>
 __device__ __forceinline__ uint32_t v_off(int row, int ch, float) { return k_off<ROWB>(row, ch); }
 
+// Tile addresses are formed as (what belongs to the lane) xor (a constant per fragment): rows are 128, 256 or 512 bytes, chunk
+// bits lie below them, and a tile starts at a multiple of 256.  One register per tile instead of one per fragment.
+template <typename V>
+__device__ __forceinline__ V lds_at(uint32_t addr) {
+  using LV = const __attribute__((address_space(3))) V;
+  return *(LV*)(uintptr_t)addr;
+}
+// k_lane: address of chunk h (bf16) or 2 h (fp32) of token c; the fragment of step ks of token 32 t + c
 template <int ROWB>
-__device__ __forceinline__ bf16x8 k_frag32(const char* kt, int row, int ks, int h, bf16) {
-  return *reinterpret_cast<const bf16x8*>(kt + k_off<ROWB>(row, 2 * ks + h));
+__device__ __forceinline__ bf16x8 k_frag32(uint32_t k_lane, int t, int ks, bf16) {
+  return lds_at<bf16x8>((k_lane ^ (uint32_t)(ks << 5)) + t * 32 * ROWB);
 }
 template <int ROWB>
-__device__ __forceinline__ f32x8 k_frag32(const char* kt, int row, int ks, int h, float) {
+__device__ __forceinline__ f32x8 k_frag32(uint32_t k_lane, int t, int ks, float) {
   f32x8 f;
-  f.lo = *reinterpret_cast<const f32x4*>(kt + k_off<ROWB>(row, 4 * ks + 2 * h));
-  f.hi = *reinterpret_cast<const f32x4*>(kt + k_off<ROWB>(row, 4 * ks + 2 * h + 1));
+  f.lo = lds_at<f32x4>((k_lane ^ (uint32_t)(ks << 6)) + t * 32 * ROWB);
+  f.hi = lds_at<f32x4>((k_lane ^ (uint32_t)(ks << 6) ^ 16u) + t * 32 * ROWB);
   return f;
 }
-// V^T of dims 32 dt .. + 31, 16-token step s: element j of lane (h, c) is V[16 s + 8 (j >> 2) + 4 h + (j & 3)][32 dt + c]
+// V^T of dims 32 dt .. + 31, 16-token step s: element j of lane (h, c) is V[16 s + 8 (j >> 2) + 4 h + (j & 3)][32 dt + c].
+// v_lane (bf16): address of this lane's 8 bytes of step 0, dims 0 .. 31.
 template <int ROWB>
-__device__ __forceinline__ bf16x8 v_frag32(const char* vt, int dt, int s, int lane, bf16) {
+__device__ __forceinline__ bf16x8 v_frag32(uint32_t v_lane, int dt, int s, int lane, bf16) {
   using lds_bf16x4 = __attribute__((address_space(3))) bf16x4;
-  const int h = lane >> 5, half = (lane >> 4) & 1, r = lane & 15;
   bf16x8 f;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int key = 16 * s + 8 * u + 4 * h + (r >> 2);
-    const char* p = vt + v_off<ROWB>(key, 4 * dt + 2 * half + ((r & 3) >> 1), bf16{}) + 8 * (r & 1);
-    const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(p));
+    const bf16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(uintptr_t)((v_lane ^ (uint32_t)(dt << 6)) + (16 * s + 8 * u) * ROWB));
 #pragma unroll
     for (int q = 0; q < 4; ++q) f[4 * u + q] = v[q];
   }
   return f;
 }
 template <int ROWB>
-__device__ __forceinline__ f32x8 v_frag32(const char* vt, int dt, int s, int lane, float) {
+__device__ __forceinline__ f32x8 v_frag32(uint32_t v_tile, int dt, int s, int lane, float) {
   const int h = lane >> 5, d = 32 * dt + (lane & 31);
   f32x8 f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int key = 16 * s + 8 * (j >> 2) + 4 * h + (j & 3);
-    const float v = *reinterpret_cast<const float*>(vt + v_off<ROWB>(key, d >> 2, float{}) + 4 * (d & 3));
+    const float v = lds_at<float>(v_tile + v_off<ROWB>(key, d >> 2, float{}) + 4 * (d & 3));
     if (j < 4) f.lo[j] = v; else f.hi[j - 4] = v;
   }
   return f;
@@ -452,7 +487,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   using Frag = typename Traits<T>::Frag;
   constexpr int ROWB = TL::ROWB, CPR = TL::CPR, ES = (int)sizeof(T);
   constexpr int KS = DP / 16, NDT = DP / 32, NL = CPR / 4, RPI = 64 / CPR;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(1024))) char tiles[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int h = lane >> 5, c = lane & 31;
@@ -465,8 +500,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   const int group = a.heads / a.kv_heads;
 
   TileInfo ti;
-  if (!find_tile(a, tile, tt, ti)) return;
-  if (sp.share == 2 && !is_chunk(a, ti, group)) return;
+  if (!find_tile(a, tile, sp, ti)) return;
   const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
   const int live_tt = ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt;
   const int last = first + live_tt - 1;
@@ -518,27 +552,42 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
 
   u32x4 kr[NL], vr[NL];
   int ok = 0;
+  // this lane's piece of the first rows of 16 tokens; outside for dims past the head's (and then also RPI.. rows further on)
+  const bool pad = (lane % CPR) * 16 >= a.dim * ES;
+  const uint32_t koff = pad ? OOB : (uint32_t)(lane / CPR * a.k_slot + lane % CPR * 16);
+  const uint32_t voff = pad ? OOB : (uint32_t)(lane / CPR * a.v_slot + lane % CPR * 16);
   auto tile_of = [&](int i) { return i < sb ? i : lot + i - sb; };
-  auto fetch = [&](int i) {
+  // page of this wave's 16 tokens of a tile (-1 behind hi), left in a vector register until the tile is fetched: made
+  // uniform at once, the wait for it would also wait for the tile's loads in front of it
+  auto page_of = [&](int i) {
     const int tok0 = tile_of(i) * 64 + 16 * wave;
-    int left = hi - tok0;
-    left = left > 16 ? 16 : left;
-    int page = -1;
-    if (left > 0) page = uniform(trow[tok0 >> a.shift]);
-    const bool good = page >= 0 && page < a.n_pages;
-    ok = good || left <= 0;
-    const int slot0 = tok0 & ((1 << a.shift) - 1);
-    const char* kp = kbase + (long long)(good ? page : 0) * a.k_page + (long long)slot0 * a.k_slot;
-    const char* vp = vbase + (long long)(good ? page : 0) * a.v_page + (long long)slot0 * a.v_slot;
+    return i < i1 && tok0 < hi ? trow[tok0 >> a.shift] : -1;
+  };
+  auto fetch = [&](int i, int vpage) {
+    const int page = uniform(vpage);
+    const int tok0 = tile_of(i) * 64 + 16 * wave;
+    const int left = hi - tok0 > 16 ? 16 : hi - tok0;
+    const bool good = ((unsigned)page < (unsigned)a.n_pages) & (left > 0);
+    ok = good | (left <= 0);
+    const uint32_t slot0 = tok0 & ((1 << a.shift) - 1), p0 = good ? page : 0;
+    const char* kp = kbase + (unsigned long long)p0 * (uint32_t)a.k_page + slot0 * (uint32_t)a.k_slot;
+    const char* vp = vbase + (unsigned long long)p0 * (uint32_t)a.v_page + slot0 * (uint32_t)a.v_slot;
     const __amdgpu_buffer_rsrc_t kd = buffer_of(kp, good ? (left - 1) * a.k_slot + a.dim * ES : 0);
     const __amdgpu_buffer_rsrc_t vd = buffer_of(vp, good ? (left - 1) * a.v_slot + a.dim * ES : 0);
+    if (tok0 < lo) {                                         // may hold tokens between the sinks and the window: nobody sees those
 #pragma unroll
-    for (int v = 0; v < NL; ++v) {
-      const int row = v * RPI + lane / CPR, ch = lane % CPR;
-      // nobody sees the tokens between the sinks and the window
-      const bool dead = ch * 16 >= a.dim * ES || (tok0 + row < lo && tok0 + row >= sinks);
-      kr[v] = __builtin_amdgcn_raw_buffer_load_b128(kd, (int)(dead ? OOB : (uint32_t)(row * a.k_slot + ch * 16)), 0, 0);
-      vr[v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(dead ? OOB : (uint32_t)(row * a.v_slot + ch * 16)), 0, 0);
+      for (int v = 0; v < NL; ++v) {
+        const int j = tok0 + v * RPI + lane / CPR;
+        const bool dead = (j < lo) & (j >= sinks);
+        kr[v] = __builtin_amdgcn_raw_buffer_load_b128(kd, (int)(dead ? OOB : koff + (uint32_t)(v * RPI * a.k_slot)), 0, 0);
+        vr[v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(dead ? OOB : voff + (uint32_t)(v * RPI * a.v_slot)), 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < NL; ++v) {
+        kr[v] = __builtin_amdgcn_raw_buffer_load_b128(kd, (int)(koff + (uint32_t)(v * RPI * a.k_slot)), 0, 0);
+        vr[v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(voff + (uint32_t)(v * RPI * a.v_slot)), 0, 0);
+      }
     }
   };
   auto commit = [&](char* st) {
@@ -551,28 +600,63 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
     if (lane == 0) reinterpret_cast<int*>(st + TL::OK_OFF)[wave] = ok;
   };
 
+  int page = page_of(i0);
   if (i0 < i1) {
-    fetch(i0);
-    commit(smem);
+    fetch(i0, page);
+    page = page_of(i0 + 1);
+    commit(tiles);
   }
+  __builtin_amdgcn_s_waitcnt(0x0f70);    // vmcnt(0): q has arrived, said once, or every first product in the loop would wait for the tile on its way
   for (int i = i0; i < i1; ++i) {
-    char* st = smem + (TL::NST == 2 ? (i - i0) & 1 : 0) * TL::STAGE;
+    char* st = tiles + (TL::NST == 2 ? (i - i0) & 1 : 0) * TL::STAGE;
     __syncthreads();
     const bool more = i + 1 < i1;
-    if (more) fetch(i + 1);
+    if (more) {
+      fetch(i + 1, page);
+      page = page_of(i + 2);
+    }
     const int j0 = tile_of(i) * 64;
     // a wave skips tiles that none of its rows sees
     bool sees = busy && (!a.causal || j0 <= wlast);
     if (a.window > 0) sees = sees && (j0 + 63 >= wfirst - a.window + 1 || j0 < sinks);
     if (sees) {
       const u32x4 okv = *reinterpret_cast<const u32x4*>(st + TL::OK_OFF);
+      // all fragments of 32 tokens are on their way before the first product; the next 32 tokens' replace them one by one
       f32x16 s[2];
+      Frag kf[KS];
+      const uint32_t st_at = (uint32_t)(uintptr_t)st, k_lane = st_at + k_off<ROWB>(c, sizeof(T) == 2 ? h : 2 * h);
+      uint32_t v_lane = st_at + TL::V_OFF;
+      if constexpr (sizeof(T) == 2) {
+        const int r = lane & 15;
+        v_lane += v_off<ROWB>(4 * h + (r >> 2), 2 * ((lane >> 4) & 1) + ((r & 3) >> 1), T{}) + 8 * (r & 1);
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[ks] = k_frag32<ROWB>(k_lane, 0, ks, T{});
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) mma32(s[t], k_frag32<ROWB>(st, 32 * t + c, ks, h, T{}), q[ks]);
+        for (int ks = 0; ks < KS; ++ks) {
+          mma32(s[t], kf[ks], q[ks]);
+          if (t == 0) kf[ks] = k_frag32<ROWB>(k_lane, 1, ks, T{});
+        }
+      }
+      Frag vf[NDT];
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) vf[dt] = v_frag32<ROWB>(v_lane, dt, 0, lane, T{});
+      if constexpr (sizeof(T) == 2) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1 + KS, 0);          // LDS reads
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // one product, one read
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
       }
       bool inside = uniform(okv[0] & okv[1] & okv[2] & okv[3]) && j0 + 63 <= (a.causal ? wfirst : ti.kv - 1);
       if (a.window > 0) inside = inside && (j0 >= wlast - a.window + 1 || j0 + 63 < sinks);
@@ -617,13 +701,26 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         // rounded to the storage type for the product; the sum is not
         const Frag pf = p_frag(pk, T{});
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) mma32(ot[dt], v_frag32<ROWB>(st + TL::V_OFF, dt, u, lane, T{}), pf);
+        for (int dt = 0; dt < NDT; ++dt) {
+          mma32(ot[dt], vf[dt], pf);
+          if (u < 3) vf[dt] = v_frag32<ROWB>(v_lane, dt, u + 1, lane, T{});
+        }
+        if constexpr (sizeof(T) == 2) {
+          if (u < 3) {                                       // the next step's exponentials run beside the products
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 28 / NDT, 0);
+            }
+          }
+        }
       }
       l_run += psum;
     }
     if (more) {
       if (TL::NST == 1) __syncthreads();
-      commit(smem + (TL::NST == 2 ? (i + 1 - i0) & 1 : 0) * TL::STAGE);
+      commit(tiles + (TL::NST == 2 ? (i + 1 - i0) & 1 : 0) * TL::STAGE);
     }
   }
 
@@ -634,7 +731,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   }
   if (!live) return;
   const long long orow = (long long)(ti.c0 + ti.t0 + rt) * a.heads + kvh * group + rh;
-  if (sp.ws_pieces == 1) {
+  if (sp.pieces == 1) {
     const float inv = l_run > 0.f ? 1.0f / l_run : (l_run == 0.f ? 0.f : l_run);       // NaN stays NaN
     T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
 #pragma unroll
@@ -645,8 +742,8 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         if (d < a.dim) store4(o + d, f32x4{ot[dt][4 * e], ot[dt][4 * e + 1], ot[dt][4 * e + 2], ot[dt][4 * e + 3]} * inv);
       }
   } else {
-    const long long rows = (long long)a.rows * a.heads;
-    float* o = a.ws + ws_sums(rows, sp.ws_pieces) + (orow * sp.ws_pieces + split) * a.dim;
+    const long long at = ws_row(a, sp, ti, ti.t0 + rt, kvh * group + rh) * sp.pieces + split;
+    float* o = a.ws + sp.ws + ws_sums(sp.ws_rows, sp.pieces) + at * a.dim;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -654,44 +751,72 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         const int d = 32 * dt + 8 * e + 4 * h;
         if (d < a.dim) store4(o + d, f32x4{ot[dt][4 * e], ot[dt][4 * e + 1], ot[dt][4 * e + 2], ot[dt][4 * e + 3]});
       }
-    if (h == 0) {
-      float2* out = reinterpret_cast<float2*>(a.ws) + orow * sp.ws_pieces;
-      out[split] = float2{m_run * cs, l_run};                // the join works in base-2 exponents
-      if (split == 0)
-        for (int i = sp.pieces; i < sp.ws_pieces; ++i) out[i] = float2{-INFINITY, 0.f};
-    }
+    if (h == 0) reinterpret_cast<float2*>(a.ws + sp.ws)[at] = float2{m_run * cs, l_run};    // the join works in base-2 exponents
   }
 }
 
-// joins the pieces of a split key axis: one wave per (row, head)
+// Joins the pieces of a launch's split key axis: a workgroup per (row, head) of its share.  32 threads hold the dims, four
+// each; the eight groups of 32 take every eighth piece, four loads in flight, and meet in LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs a, int splits) {
-  const long long rows = (long long)a.rows * a.heads;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  float2 p{-INFINITY, 0.f};
-  if (lane < splits) p = reinterpret_cast<const float2*>(a.ws)[row * splits + lane];
+__global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs a, const Split sp) {
+  __shared__ float s_m[4], s_l[4];
+  __shared__ float s_w[MAX_SPLITS];
+  __shared__ f32x4 s_acc[8][32];
+  const int at = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = sp.pieces;
+  const int wrow = at / a.heads, head = at - wrow * a.heads;
+  int row = wrow;
+  if (sp.share == 1) {
+    const int b = wrow / sp.per_request, i = wrow - b * sp.per_request;
+    const int c0 = clamp_rows(a.cu_rows[b], a.rows), n = clamp_rows(a.cu_rows[b + 1], a.rows) - c0;
+    if (i >= n || n > sp.per_request) return;
+    row = c0 + i;
+  } else if (sp.share == 2) {
+    int lo = 0, hi = a.B + 1;                                // the request of this row (B: behind the last one)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu_rows[mid] <= row) lo = mid; else hi = mid;
+    }
+    if (lo < a.B && clamp_rows(a.cu_rows[lo + 1], a.rows) - clamp_rows(a.cu_rows[lo], a.rows) <= sp.per_request) return;
+  }
+  float2 p{-INFINITY, 0.f};                                  // MAX_SPLITS pieces: one per thread
+  if (tid < pieces) p = reinterpret_cast<const float2*>(a.ws + sp.ws)[(long long)at * pieces + tid];
   float m = p.x;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  const float f = p.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.x - m);
+  if (lane == 0) s_m[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float f = p.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.x - m);     // a piece that saw nothing has no part
   float l = p.y * f;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+  if (lane == 0) s_l[wave] = l;
+  s_w[tid] = f;
+  __syncthreads();
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
   const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  const float* src = a.ws + ws_sums(rows, splits) + row * splits * a.dim;
-  float acc[2] = {0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const float w = __shfl(f, s);
-    if (w == 0.f) continue;                                  // a piece that saw nothing
+  const int g = tid >> 5, d = (tid & 31) * 4;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (d < a.dim) {
+    const float* src = a.ws + sp.ws + ws_sums(sp.ws_rows, pieces) + (long long)at * pieces * a.dim + d;
+    for (int k0 = g; k0 < pieces; k0 += 32) {
+      f32x4 v[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (lane + 64 * k < a.dim) acc[k] += w * src[(long long)s * a.dim + lane + 64 * k];
+      for (int k = 0; k < 4; ++k) {
+        v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (k0 + 8 * k < pieces) v[k] = *reinterpret_cast<const f32x4*>(src + (long long)(k0 + 8 * k) * a.dim);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k0 + 8 * k < pieces) acc += v[k] * s_w[k0 + 8 * k];
+    }
   }
+  s_acc[g][tid & 31] = acc;
+  __syncthreads();
+  if (g != 0 || d >= a.dim) return;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (lane + 64 * k < a.dim) store_row(reinterpret_cast<T*>(a.out) + row * a.dim + lane + 64 * k, acc[k] * inv);
+  for (int k = 1; k < 8; ++k) acc += s_acc[k][tid & 31];
+  store4(reinterpret_cast<T*>(a.out) + ((long long)row * a.heads + head) * a.dim + d, acc * inv);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -699,8 +824,8 @@ __global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs 
 // ---------------------------------------------------------------------------------------------------------------
 struct Plan {
   Split step, chunk;
-  int step_tiles = 0, chunk_tiles = 0;                       // chunk_tiles 0: not launched
-  int pieces = 1;
+  long long step_tiles = 0, chunk_tiles = 0;                 // 0: not launched
+  long long ws = 0;                                          // floats
 };
 
 // pieces of the key axis that give a launch `want` workgroups, none shorter than `least` tokens for the longest request
@@ -715,45 +840,44 @@ int pieces_for(const PageAttnArgs& a, long long busy, long long want, int least)
   return n < 1 ? 1 : (int)n;
 }
 
+long long ws_floats(const PageAttnArgs& a, const Split& s) {
+  return s.pieces > 1 ? ws_sums(s.ws_rows, s.pieces) + s.ws_rows * s.pieces * a.dim : 0;
+}
+
 Plan make_plan(const PageAttnArgs& a) {
   Plan p;
   const int group = a.heads / a.kv_heads;
+  const int few = CHUNK_MIN / group;                                                          // rows of a short request
   const long long longest = a.max_rows > 0 && a.max_rows < a.rows ? a.max_rows : a.rows;      // rows of one request
-  const bool chunks = longest * group > CHUNK_MIN;
-  // without a hint a batch of as many rows as requests is taken for single tokens (the chunk kernel would find nothing)
-  const bool only_steps = !chunks || (a.max_rows == 0 && a.rows <= a.B);
-  const long long some = a.rows < a.B ? a.rows : a.B;
-  {
+  // without a hint a batch of as many rows as requests is taken for single tokens
+  const bool chunks = longest > few && (a.max_rows > 0 || a.rows > a.B || few == 0);
+  if (few > 0 || !chunks) {
     Split& s = p.step;
     s.gc = group < STEP_ROWS ? group : STEP_ROWS;
     s.hchunks = (group + s.gc - 1) / s.gc;
     s.tt = STEP_ROWS / s.gc;
-    s.share = only_steps ? 0 : 1;
-    p.step_tiles = a.rows / s.tt + a.B + 1;
-    const long long full = only_steps ? (a.rows + s.tt - 1) / s.tt : some;
-    s.pieces = pieces_for(a, (full > some ? full : some) * a.kv_heads * s.hchunks, 1024, 256);
+    s.share = chunks ? 1 : 0;
+    s.per_request = chunks ? few : 0;
+    p.step_tiles = chunks ? (long long)a.B * ((few + s.tt - 1) / s.tt) : (long long)a.rows / s.tt + a.B + 1;
+    const long long full = chunks ? 0 : (a.rows + s.tt - 1) / s.tt, some = a.rows < a.B ? a.rows : a.B;
+    s.pieces = pieces_for(a, (full > some ? full : some) * a.kv_heads * s.hchunks, 2048, 256);
+    s.ws_rows = (chunks ? (long long)a.B * few : (long long)a.rows) * a.heads;
   }
-  p.pieces = p.step.pieces;
-  if (!only_steps) {
+  if (chunks) {
     Split& s = p.chunk;
     s.gc = group < CHUNK_ROWS ? group : CHUNK_ROWS;
     s.hchunks = (group + s.gc - 1) / s.gc;
     s.tt = CHUNK_ROWS / s.gc;
     s.share = 2;
-    p.chunk_tiles = a.rows / s.tt + a.B + 1;
-    s.pieces = pieces_for(a, (a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 1024, 512);
-    if (s.pieces > p.pieces) p.pieces = s.pieces;
+    s.per_request = few;
+    p.chunk_tiles = (long long)a.rows / s.tt + a.B + 1;
+    s.pieces = pieces_for(a, (long long)(a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 2048, 512);
+    s.ws_rows = (long long)a.rows * a.heads;
+    s.ws = (ws_floats(a, p.step) + 3) & ~3ll;
   }
-  p.step.ws_pieces = p.chunk.ws_pieces = p.pieces;
+  p.ws = p.chunk.ws + ws_floats(a, p.chunk);
+  if (p.chunk_tiles == 0) p.ws = ws_floats(a, p.step);
   return p;
-}
-
-long long chunk_grid(const PageAttnArgs& a, const Plan& p) { return (long long)p.chunk_tiles * a.kv_heads * p.chunk.hchunks; }
-
-size_t split_bytes(const PageAttnArgs& a, int pieces) {
-  if (pieces <= 1) return 0;
-  const long long rows = (long long)a.rows * a.heads;
-  return (size_t)(ws_sums(rows, pieces) + rows * pieces * a.dim) * sizeof(float);
 }
 
 int check_args(int dtype, const PageAttnArgs& a) {
@@ -769,9 +893,17 @@ int check_args(int dtype, const PageAttnArgs& a) {
   const long long strides[] = {a.q_row, a.q_head, a.k_page, a.k_head, a.k_slot, a.v_page, a.v_head, a.v_slot};
   for (long long s : strides)
     if (s % 16) return fail("page_attention: strides must be multiples of 16 bytes");
-  if (a.k_slot < a.dim * es || a.v_slot < a.dim * es || a.k_slot > (1 << 26) || a.v_slot > (1 << 26)) return fail("page_attention: slots of %d / %d bytes for %d dims", a.k_slot, a.v_slot, a.dim);
+  if (a.k_slot < a.dim * es || a.v_slot < a.dim * es || a.k_slot > (1 << 24) || a.v_slot > (1 << 24)) return fail("page_attention: slots of %d / %d bytes for %d dims", a.k_slot, a.v_slot, a.dim);
+  // page and slot offsets are formed in 32 bits, addresses in 64
+  if (a.k_page < 0 || a.v_page < 0 || a.k_page > 0xffffffffll || a.v_page > 0xffffffffll) return fail("page_attention: page strides of %lld / %lld bytes (at most 2^32 - 1)", a.k_page, a.v_page);
+  if (((long long)a.k_slot << a.shift) > 0x7fffffffll || ((long long)a.v_slot << a.shift) > 0x7fffffffll) return fail("page_attention: pages of more than 2 GiB");
   if ((long long)a.rows * a.heads > 0x7fffffffll || a.kv_heads > 65535) return fail("page_attention: too many rows or heads");
   return 0;
+}
+
+template <typename T>
+void join(const PageAttnArgs& a, const Split& s, hipStream_t stream) {
+  if (s.pieces > 1) page_attn_join_kernel<T><<<(unsigned)s.ws_rows, 256, 0, stream>>>(a, s);
 }
 
 template <typename T, int DP>
@@ -780,15 +912,18 @@ int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
   using CT = ChunkTile<T, DP>;
   auto sk = page_attn_step_kernel<T, DP>;
   auto ck = page_attn_chunk_kernel<T, DP>;
+  const long long chunk_grid = p.chunk_tiles * a.kv_heads * p.chunk.hchunks;
+  if (chunk_grid > 0x7fffffffll || p.step_tiles > 0x7fffffffll || (long long)a.kv_heads * p.step.hchunks > 65535)
+    return fail("page_attention: too many rows or heads");
   if (p.chunk_tiles > 0) {
     if (reserve_lds(reinterpret_cast<const void*>(ck), CT::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", CT::BYTES);
-    ck<<<dim3((unsigned)chunk_grid(a, p), p.chunk.pieces), 256, CT::BYTES, stream>>>(a, p.chunk);
+    ck<<<dim3((unsigned)chunk_grid, p.chunk.pieces), 256, CT::BYTES, stream>>>(a, p.chunk);
+    join<T>(a, p.chunk, stream);
   }
-  if (reserve_lds(reinterpret_cast<const void*>(sk), ST::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", ST::BYTES);
-  sk<<<dim3(p.step_tiles, a.kv_heads * p.step.hchunks, p.step.pieces), 64 * STEP_WAVES, ST::BYTES, stream>>>(a, p.step);
-  if (p.pieces > 1) {
-    const long long rows = (long long)a.rows * a.heads;
-    page_attn_join_kernel<T><<<(unsigned)((rows + 3) / 4), 256, 0, stream>>>(a, p.pieces);
+  if (p.step_tiles > 0) {
+    if (reserve_lds(reinterpret_cast<const void*>(sk), ST::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", ST::BYTES);
+    sk<<<dim3((unsigned)p.step_tiles, a.kv_heads * p.step.hchunks, p.step.pieces), 64 * STEP_WAVES, ST::BYTES, stream>>>(a, p.step);
+    join<T>(a, p.step, stream);
   }
   return check_launch("page_attention");
 }
@@ -797,7 +932,7 @@ int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
 
 size_t page_attention_workspace_bytes(int dtype, const PageAttnArgs& a) {
   if (check_args(dtype, a) != 0) return 0;
-  return split_bytes(a, make_plan(a).pieces);
+  return (size_t)make_plan(a).ws * sizeof(float);
 }
 
 int launch_page_attention(int dtype, const PageAttnArgs& a, size_t ws_bytes, hipStream_t stream) {
@@ -806,9 +941,8 @@ int launch_page_attention(int dtype, const PageAttnArgs& a, size_t ws_bytes, hip
   if (!a.q || !a.k || !a.v || !a.table || !a.kv_lens || !a.cu_rows || !a.out) return fail("page_attention: null operand");
   if ((uintptr_t)a.q % 16 || (uintptr_t)a.k % 16 || (uintptr_t)a.v % 16 || (uintptr_t)a.out % 16) return fail("page_attention: operands must be 16-byte aligned");
   const Plan p = make_plan(a);
-  const size_t need = split_bytes(a, p.pieces);
+  const size_t need = (size_t)p.ws * sizeof(float);
   if (need > 0 && (!a.ws || ws_bytes < need || (uintptr_t)a.ws % 16)) return fail("page_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  if (chunk_grid(a, p) > 0x7fffffffll || (long long)a.kv_heads * p.step.hchunks > 65535) return fail("page_attention: too many rows or heads");
   if (dtype == DT_BF16) return a.dim <= 64 ? run<bf16, 64>(a, p, stream) : run<bf16, 128>(a, p, stream);
   return a.dim <= 64 ? run<float, 64>(a, p, stream) : run<float, 128>(a, p, stream);
 }

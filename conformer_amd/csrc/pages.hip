@@ -24,7 +24,6 @@ constexpr int PLAN_WAVES = PLAN_THREADS / 64;
 // Steps with up to this many rows (and PLAN_THREADS requests) find their slots in the planning workgroup itself, out of
 // LDS; longer ones leave them to a second launch over all CUs.
 constexpr int PLAN_INLINE_ROWS = 4 * PLAN_THREADS;
-constexpr int OWN_PAGES = 4;
 
 __device__ __forceinline__ long long wave_scan(long long v, int lane) {      // inclusive
 #pragma unroll
@@ -61,13 +60,26 @@ __device__ __forceinline__ long long slot_of(const int32_t* row, int pos, int sh
   return ((long long)row[pos >> shift] << shift) + (pos & ((1 << shift) - 1));
 }
 
+// the last of `n` rising starts that is at or before i (starts[0] = 0); its row is not empty if i lies before the end
+__device__ __forceinline__ int last_at(const int* starts, int n, int i) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= i) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
 // One workgroup: a plan is a chain of prefix sums over a few hundred requests, bound by latency, and one workgroup
-// needs no hand-over between CUs.  It has a thread per request or row up to PLAN_THREADS; with one wave no scan waits at a barrier.
-// A thread moves up to OWN_PAGES pages of its request by itself, a wave those of a longer one together.
+// needs no hand-over between CUs.  With one wave no scan waits at a barrier.  Pages are moved one per thread, each thread
+// finding its page's request by bisection of the prefix sums in LDS, so that a prompt of thousands of pages is spread
+// over all threads.
 __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanArgs a, int inline_slots) {
   __shared__ long long part[PLAN_WAVES];
   __shared__ int s_kv[PLAN_THREADS];                 // length before the step (0 for rows that finished), -1 if refused
   __shared__ int s_cu[PLAN_THREADS + 1];
+  __shared__ int s_take[PLAN_THREADS];               // pages moved for the rows before this one
+  __shared__ int s_held[PLAN_THREADS];
   const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x, waves = threads >> 6;
   const int cap = a.width << a.shift;                // the longest request the table can describe
   int top = *a.free_count;
@@ -84,17 +96,18 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanA
         count = pages_of(kv, a.shift);
       }
       long long total;
-      const long long first = top + block_scan(count, part, waves, total) - count;
-      const int at = first > a.pool ? a.pool : (int)first;
-      for (unsigned long long m = __ballot(count > 0); m; m &= m - 1) {
-        const int i = __ffsll(m) - 1;
-        const int n = __shfl(count, i), to = __shfl(at, i);
-        const int32_t* row = a.table + (size_t)(b - lane + i) * a.table_row;
-        for (int c = lane; c < n; c += 64)
-          if (c < a.pool - to) a.free_pages[to + c] = row[c];     // a pool never gets back more pages than it has
+      const long long before = block_scan(count, part, waves, total) - count;
+      s_take[tid] = before > 0x7fffffff ? 0x7fffffff : (int)before;
+      __syncthreads();
+      const int room = a.pool - top, rows = a.B - b0 < threads ? a.B - b0 : threads;
+      const int pushed = total < room ? (int)total : room;      // a pool never gets back more pages than it has
+#pragma unroll 4
+      for (int i = tid; i < pushed; i += threads) {
+        const int k = last_at(s_take, rows, i);
+        a.free_pages[top + i] = a.table[(size_t)(b0 + k) * a.table_row + (i - s_take[k])];
       }
-      const long long next = top + total;
-      top = next > a.pool ? a.pool : (int)next;
+      top += pushed;
+      __syncthreads();
     }
     __threadfence_block();
     __syncthreads();                                 // pages pushed are visible to the pops below
@@ -136,17 +149,16 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanA
       s_cu[tid + 1] = end;
       a.cu_rows[a.B] = end;
     }
-    const int from = top - 1 - (int)(taken - need);
-    if (need > 0 && need <= OWN_PAGES) {
-      int32_t* row = a.table + (size_t)b * a.table_row + held;
-      for (int c = 0; c < need; ++c) row[c] = a.free_pages[from - c];
+    s_take[tid] = (int)(taken - need - (taken_before - total));
+    s_held[tid] = held;
+    __syncthreads();
+    const int rows = a.B - b0 < threads ? a.B - b0 : threads, from = top - 1 - (int)(taken_before - total);
+#pragma unroll 4
+    for (int i = tid; i < (int)total; i += threads) {
+      const int k = last_at(s_take, rows, i);
+      a.table[(size_t)(b0 + k) * a.table_row + s_held[k] + (i - s_take[k])] = a.free_pages[from - i];
     }
-    for (unsigned long long m = __ballot(need > OWN_PAGES); m; m &= m - 1) {
-      const int i = __ffsll(m) - 1;
-      const int count = __shfl(need, i), f = __shfl(from, i);
-      int32_t* row = a.table + (size_t)(b - lane + i) * a.table_row + __shfl(held, i);
-      for (int c = lane; c < count; c += 64) row[c] = a.free_pages[f - c];
-    }
+    if (b0 + threads < a.B) __syncthreads();
   }
   if (tid == 0) *a.free_count = top - (int)taken_before;
 
@@ -157,11 +169,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(const PagePlanA
   for (int i = tid; i < a.rows; i += threads) {
     long long slot = -1;
     if (i < s_cu[a.B]) {
-      int lo = 0, hi = a.B;                          // the last request that starts at or before row i (it is not empty)
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_cu[mid] <= i) lo = mid; else hi = mid;
-      }
+      const int lo = last_at(s_cu, a.B, i);
       if (s_kv[lo] >= 0) slot = slot_of(a.table + (size_t)lo * a.table_row, s_kv[lo] + i - s_cu[lo], a.shift);
     }
     a.slots[i] = slot;
@@ -174,11 +182,7 @@ __global__ __launch_bounds__(256) void page_slots_kernel(const PagePlanArgs a) {
   if (i >= a.rows) return;
   long long slot = -1;
   if (i < a.cu_rows[a.B]) {
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu_rows[mid] <= i) lo = mid; else hi = mid;
-    }
+    const int lo = last_at(a.cu_rows, a.B, i);
     if (a.granted[lo]) {
       const int pos = a.kv_lens[lo] - (a.cu_rows[lo + 1] - i);        // kv_lens already counts the step's rows
       slot = slot_of(a.table + (size_t)lo * a.table_row, pos, a.shift);
@@ -221,8 +225,9 @@ int launch_page_plan(const PagePlanArgs& a, hipStream_t stream) {
   if (((long long)a.width << a.shift) > 0x7fffffffll) return fail("page_plan: a table of %d pages describes more than 2^31 - 1 tokens", a.width);
   if (!a.kv_lens || !a.new_lens || !a.table || !a.free_pages || !a.free_count || !a.cu_rows || !a.granted || (a.rows > 0 && !a.slots)) return fail("page_plan: null operand");
   const bool inl = a.B <= PLAN_THREADS && a.rows <= PLAN_INLINE_ROWS;
-  int threads = a.B > a.rows || !inl ? a.B : a.rows;
-  threads = threads > PLAN_THREADS ? PLAN_THREADS : (threads + 63) / 64 * 64;
+  // a thread per request, or per row of a short step; all of them where whole prompts or whole requests' pages may move
+  int threads = a.B > a.rows ? a.B : a.rows;
+  threads = !inl || a.finished || threads > PLAN_THREADS ? PLAN_THREADS : (threads + 63) / 64 * 64;
   page_plan_kernel<<<1, threads, 0, stream>>>(a, inl ? 1 : 0);
   if (!inl && a.rows > 0) page_slots_kernel<<<(a.rows - 1) / 256 + 1, 256, 0, stream>>>(a);
   return check_launch("page_plan");

@@ -186,7 +186,7 @@ __device__ __forceinline__ V wave_running(V v, int lane) {
 // ---- where the elements come from: the row in memory, or the list in LDS ----
 template <typename T>
 struct RowSource {
-  static constexpr int AHEAD = sizeof(T) == 2 ? 4 : 2;         // vectors in flight per lane
+  static constexpr int AHEAD = 2;         // vectors in flight per lane
   const T* row;
   int n, wave, waves, lane;
 
