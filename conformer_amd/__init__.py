@@ -10,8 +10,9 @@ from .frontend import MelSpectrogram
 from .modules import (CausalConv1d, ConformerConvolution, FastConformerBlock, FastConformerEncoder,
                       FeedForwardModule, RelativePositionalEncoding, RelPositionMultiHeadAttention, Subsampling8x,
                       stochastic_depth_schedule)
+from .paging import KVPages
 
 __all__ = ["create_model", "load_config", "model_size", "FastConformerTransducer", "FastConformerEncoder",
            "FastConformerBlock", "Subsampling8x", "RelativePositionalEncoding", "RelPositionMultiHeadAttention",
            "ConformerConvolution", "FeedForwardModule", "CausalConv1d", "StatelessPredictor", "JointNetwork",
-           "StochasticDepthConfig", "stochastic_depth_schedule", "MelSpectrogram"]
+           "StochasticDepthConfig", "stochastic_depth_schedule", "MelSpectrogram", "KVPages"]

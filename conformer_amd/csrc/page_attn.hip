@@ -183,12 +183,17 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int gc = sp.gc, tt = sp.tt, split = blockIdx.z;
-  const int kvh = blockIdx.y / sp.hchunks, hc = blockIdx.y - kvh * sp.hchunks;
+  const int gc = sp.gc, tt = sp.tt;
+  // pieces fastest, tiles slowest: workgroups go round the 8 XCDs by their number, and with the tile (of which some are
+  // empty) in front, a batch of two requests left half of the XCDs without work (164 against 100 us at 2 x 131072 tokens)
+  const unsigned per_tile = a.kv_heads * sp.hchunks * sp.pieces;
+  const int tile = (int)(blockIdx.x / per_tile);
+  const int rest = (int)(blockIdx.x - tile * per_tile), column = rest / sp.pieces, split = rest - column * sp.pieces;
+  const int kvh = column / sp.hchunks, hc = column - kvh * sp.hchunks;
   const int group = a.heads / a.kv_heads;
 
   TileInfo ti;
-  if (!find_tile(a, blockIdx.x, sp, ti)) return;
+  if (!find_tile(a, tile, sp, ti)) return;
   const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
   const int last = first + (ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt) - 1;
   int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
@@ -828,14 +833,19 @@ struct Plan {
   long long ws = 0;                                          // floats
 };
 
-// pieces of the key axis that give a launch `want` workgroups, none shorter than `least` tokens for the longest request
-// that the table can describe
-int pieces_for(const PageAttnArgs& a, long long busy, long long want, int least) {
+// Pieces of the key axis for a launch with `busy` workgroups per piece, by the longest request that the table can
+// describe: enough to fill the chip with `fill` workgroups as long as a piece has 256 tokens, and up to 2048, which the
+// dispatcher can balance, as long as it has `least`.  Measured on single tokens (16 rows a tile, fill 512 = two per CU, least 2048):
+// 2 requests of up to 131072 tokens x 4 kv heads 77 us with 64 pieces, 90 with 256; 64 x 8192 x 8 262 us with 4, 272 with 2.
+int pieces_for(const PageAttnArgs& a, long long busy, int fill, int least) {
   long long longest = (long long)a.width << a.shift;
   const long long seen = (long long)a.window + a.sinks + CHUNK_ROWS;
   if (a.window > 0 && seen < longest) longest = seen;
-  long long n = want / (busy > 0 ? busy : 1);
-  if (n > longest / least) n = longest / least;
+  if (busy < 1) busy = 1;
+  long long n = fill / busy, m = 2048 / busy;
+  if (n > longest / 256) n = longest / 256;
+  if (m > longest / least) m = longest / least;
+  if (m > n) n = m;
   if (n > MAX_SPLITS) n = MAX_SPLITS;
   return n < 1 ? 1 : (int)n;
 }
@@ -860,7 +870,7 @@ Plan make_plan(const PageAttnArgs& a) {
     s.per_request = chunks ? few : 0;
     p.step_tiles = chunks ? (long long)a.B * ((few + s.tt - 1) / s.tt) : (long long)a.rows / s.tt + a.B + 1;
     const long long full = chunks ? 0 : (a.rows + s.tt - 1) / s.tt, some = a.rows < a.B ? a.rows : a.B;
-    s.pieces = pieces_for(a, (full > some ? full : some) * a.kv_heads * s.hchunks, 2048, 256);
+    s.pieces = pieces_for(a, (full > some ? full : some) * a.kv_heads * s.hchunks, 512, 2048);
     s.ws_rows = (chunks ? (long long)a.B * few : (long long)a.rows) * a.heads;
   }
   if (chunks) {
@@ -871,7 +881,7 @@ Plan make_plan(const PageAttnArgs& a) {
     s.share = 2;
     s.per_request = few;
     p.chunk_tiles = (long long)a.rows / s.tt + a.B + 1;
-    s.pieces = pieces_for(a, (long long)(a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 2048, 512);
+    s.pieces = pieces_for(a, (long long)(a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 512, 2048);
     s.ws_rows = (long long)a.rows * a.heads;
     s.ws = (ws_floats(a, p.step) + 3) & ~3ll;
   }
@@ -913,7 +923,8 @@ int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
   auto sk = page_attn_step_kernel<T, DP>;
   auto ck = page_attn_chunk_kernel<T, DP>;
   const long long chunk_grid = p.chunk_tiles * a.kv_heads * p.chunk.hchunks;
-  if (chunk_grid > 0x7fffffffll || p.step_tiles > 0x7fffffffll || (long long)a.kv_heads * p.step.hchunks > 65535)
+  const long long step_grid = p.step_tiles * a.kv_heads * p.step.hchunks * p.step.pieces;
+  if (chunk_grid > 0x7fffffffll || step_grid > 0x7fffffffll)
     return fail("page_attention: too many rows or heads");
   if (p.chunk_tiles > 0) {
     if (reserve_lds(reinterpret_cast<const void*>(ck), CT::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", CT::BYTES);
@@ -922,7 +933,7 @@ int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
   }
   if (p.step_tiles > 0) {
     if (reserve_lds(reinterpret_cast<const void*>(sk), ST::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", ST::BYTES);
-    sk<<<dim3((unsigned)p.step_tiles, a.kv_heads * p.step.hchunks, p.step.pieces), 64 * STEP_WAVES, ST::BYTES, stream>>>(a, p.step);
+    sk<<<(unsigned)step_grid, 64 * STEP_WAVES, ST::BYTES, stream>>>(a, p.step);
     join<T>(a, p.step, stream);
   }
   return check_launch("page_attention");
