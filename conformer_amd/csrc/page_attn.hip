@@ -685,15 +685,18 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         swap_halves32(tmax, x, y);
         tmax = fmaxf(x, y);
       }
-      const float m_new = fmaxf(m_run, tmax);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new * cs;
-      if (__any(m_new > m_run)) {                            // the maximum seldom moves once a few tiles have gone by
-        const float alpha = __builtin_amdgcn_exp2f(m_run * cs - m_use);
+      // The reference point of the exponents follows the maximum only when it lags by more than 2^8: with 32 rows a wave the
+      // maximum of some row moves in most tiles, and every move costs a multiplication per accumulator (a third of
+      // the vector work).  Sums of terms up to 2^8 are as good in fp32, and the rounding of p is relative.
+      if (__any((tmax - m_run) * cs > 8.f)) {
+        const float m_new = fmaxf(m_run, tmax);
+        const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) * cs);
         l_run *= alpha;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) ot[dt] *= alpha;
         m_run = m_new;
       }
+      const float m_use = m_run == -INFINITY ? 0.f : m_run * cs;
       float psum = 0.f;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
