@@ -417,11 +417,10 @@ struct ChunkTile {
   static constexpr int ROWB = DP * (int)sizeof(T);
   static constexpr int CPR = ROWB / 16;
   static constexpr int KT = 64;                                  // tokens of a tile
-  static constexpr int V_OFF = KT * ROWB;
-  static constexpr int OK_OFF = 2 * KT * ROWB;                   // 4 flags: the page of every 16 tokens exists
-  static constexpr int STAGE = OK_OFF + 256;                     // keeps 256-byte rows aligned: see lds_at
-  static constexpr int NST = sizeof(T) == 2 ? 2 : 1;             // fp32 tiles are twice as large: one stage, two barriers
-  static constexpr int BYTES = NST * STAGE;
+  static constexpr int TILE = KT * ROWB;
+  static constexpr int V_OFF = 2 * TILE;                         // two K tiles, two V tiles; all at multiples of 256: see lds_at
+  static constexpr int OK_OFF = 4 * TILE;                        // 2 x 4 flags: the page of every 16 tokens exists
+  static constexpr int BYTES = OK_OFF + 32;
 };
 
 // Where 16-byte piece `ch` of row `row` lies, so that reads spread over the 256 bytes of the 64 LDS banks.  K: 16 rows that are
@@ -484,6 +483,19 @@ __device__ __forceinline__ f32x8 v_frag32(uint32_t v_tile, int dt, int s, int la
   }
   return f;
 }
+
+// 16 bytes per lane from memory to 1 KiB of LDS at `dst`, lane after lane, without a register on the way.  Written as
+// assembly because the compiler, which cannot tell the LDS tiles apart, would wait for such a load before every LDS
+// read; nothing but lds_loads_done and the barrier behind it says that the data is there.  There is no result register that
+// could be written late; the s_nop is the wait state between a write of m0 and its use here.
+__device__ __forceinline__ void lds_load16(uint32_t dst, const char* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void lds_load16(uint32_t dst, const char* src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+__device__ __forceinline__ void lds_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ const u32x4 zero16 = {0, 0, 0, 0};
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
@@ -555,115 +567,109 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
 
-  u32x4 kr[NL], vr[NL];
-  int ok = 0;
-  // this lane's piece of the first rows of 16 tokens; outside for dims past the head's (and then also RPI.. rows further on)
-  const bool pad = (lane % CPR) * 16 >= a.dim * ES;
-  const uint32_t koff = pad ? OOB : (uint32_t)(lane / CPR * a.k_slot + lane % CPR * 16);
-  const uint32_t voff = pad ? OOB : (uint32_t)(lane / CPR * a.v_slot + lane % CPR * 16);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)tiles;
   auto tile_of = [&](int i) { return i < sb ? i : lot + i - sb; };
-  // page of this wave's 16 tokens of a tile (-1 behind hi), left in a vector register until the tile is fetched: made
-  // uniform at once, the wait for it would also wait for the tile's loads in front of it
+  // page of this wave's 16 tokens of a tile (-1 behind hi), left in a vector register until it is needed: made uniform at
+  // once, the wait for it would also wait for the tile's loads in front of it
   auto page_of = [&](int i) {
     const int tok0 = tile_of(i) * 64 + 16 * wave;
     return i < i1 && tok0 < hi ? trow[tok0 >> a.shift] : -1;
   };
-  auto fetch = [&](int i, int vpage) {
-    const int page = uniform(vpage);
+  // Where lane l's 16 bytes of load v come from: LDS position l % CPR of row v RPI + l / CPR holds another piece of that row
+  uint32_t koff[NL], voff[NL];
+#pragma unroll
+  for (int v = 0; v < NL; ++v) {
+    const int row = v * RPI + lane / CPR;
+    koff[v] = (uint32_t)(row * a.k_slot) + (k_off<ROWB>(row, lane % CPR) - row * ROWB);
+    voff[v] = (uint32_t)(row * a.v_slot) + (v_off<ROWB>(row, lane % CPR, T{}) - row * ROWB);
+  }
+  // this wave's 16 tokens of K or V of tile i into LDS; true if their page exists (or none is needed)
+  auto fetch = [&](uint32_t lds_tile, int i, int page, const char* base, unsigned long long page_bytes, int slot, const uint32_t (&off)[NL]) {
     const int tok0 = tile_of(i) * 64 + 16 * wave;
-    const int left = hi - tok0 > 16 ? 16 : hi - tok0;
+    const int left = hi - tok0;
     const bool good = ((unsigned)page < (unsigned)a.n_pages) & (left > 0);
-    ok = good | (left <= 0);
     const uint32_t slot0 = tok0 & ((1 << a.shift) - 1), p0 = good ? page : 0;
-    const char* kp = kbase + (unsigned long long)p0 * (uint32_t)a.k_page + slot0 * (uint32_t)a.k_slot;
-    const char* vp = vbase + (unsigned long long)p0 * (uint32_t)a.v_page + slot0 * (uint32_t)a.v_slot;
-    const __amdgpu_buffer_rsrc_t kd = buffer_of(kp, good ? (left - 1) * a.k_slot + a.dim * ES : 0);
-    const __amdgpu_buffer_rsrc_t vd = buffer_of(vp, good ? (left - 1) * a.v_slot + a.dim * ES : 0);
-    if (tok0 < lo) {                                         // may hold tokens between the sinks and the window: nobody sees those
+    const char* src = base + p0 * page_bytes + slot0 * (uint32_t)slot;
+    const uint32_t dst = lds_tile + 16 * wave * ROWB;
+    if (good & (left >= 16) & (tok0 >= lo) & (a.dim == DP)) {
+#pragma unroll
+      for (int v = 0; v < NL; ++v) lds_load16(dst + v * 1024, src, off[v]);
+    } else {                                                 // what nobody sees comes from a row of zeros
 #pragma unroll
       for (int v = 0; v < NL; ++v) {
-        const int j = tok0 + v * RPI + lane / CPR;
-        const bool dead = (j < lo) & (j >= sinks);
-        kr[v] = __builtin_amdgcn_raw_buffer_load_b128(kd, (int)(dead ? OOB : koff + (uint32_t)(v * RPI * a.k_slot)), 0, 0);
-        vr[v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(dead ? OOB : voff + (uint32_t)(v * RPI * a.v_slot)), 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int v = 0; v < NL; ++v) {
-        kr[v] = __builtin_amdgcn_raw_buffer_load_b128(kd, (int)(koff + (uint32_t)(v * RPI * a.k_slot)), 0, 0);
-        vr[v] = __builtin_amdgcn_raw_buffer_load_b128(vd, (int)(voff + (uint32_t)(v * RPI * a.v_slot)), 0, 0);
+        const int row = v * RPI + lane / CPR, j = tok0 + row;
+        const uint32_t piece = off[v] - (uint32_t)(row * slot);
+        const bool dead = !good | (row >= left) | ((j < lo) & (j >= sinks)) | ((int)piece >= a.dim * ES);
+        lds_load16(dst + v * 1024, dead ? reinterpret_cast<const char*>(&zero16) : src + off[v]);
       }
     }
+    return good | (left <= 0);
   };
-  auto commit = [&](char* st) {
-#pragma unroll
-    for (int v = 0; v < NL; ++v) {
-      const int row = 16 * wave + v * RPI + lane / CPR, ch = lane % CPR;
-      *reinterpret_cast<u32x4*>(st + k_off<ROWB>(row, ch)) = kr[v];
-      *reinterpret_cast<u32x4*>(st + TL::V_OFF + v_off<ROWB>(row, ch, T{})) = vr[v];
-    }
-    if (lane == 0) reinterpret_cast<int*>(st + TL::OK_OFF)[wave] = ok;
+  auto fetch_k = [&](int buf, int i, int page) {
+    const bool ok = fetch(lds0 + buf * TL::TILE, i, page, kbase, (uint32_t)a.k_page, a.k_slot, koff);
+    if (lane == 0) reinterpret_cast<int*>(tiles + TL::OK_OFF + 16 * buf)[wave] = ok;
+  };
+  auto fetch_v = [&](int buf, int i, int page) {
+    fetch(lds0 + TL::V_OFF + buf * TL::TILE, i, page, vbase, (uint32_t)a.v_page, a.v_slot, voff);
+  };
+  const uint32_t k_lane = lds0 + k_off<ROWB>(c, sizeof(T) == 2 ? h : 2 * h);
+  uint32_t v_lane = lds0 + TL::V_OFF;
+  if constexpr (sizeof(T) == 2) {
+    const int r = lane & 15;
+    v_lane += v_off<ROWB>(4 * h + (r >> 2), 2 * ((lane >> 4) & 1) + ((r & 3) >> 1), T{}) + 8 * (r & 1);
+  }
+  auto flags = [&](int buf) {
+    const u32x4 f = *reinterpret_cast<const u32x4*>(tiles + TL::OK_OFF + 16 * buf);
+    return uniform((int)(f[0] | f[1] << 1 | f[2] << 2 | f[3] << 3));
   };
 
-  int page = page_of(i0);
+  // Tile i + 1's scores are formed beside tile i's softmax: the products of one fill the time that the exponentials of the
+  // other take.  K therefore runs a tile ahead of V.
+  f32x16 s[2];
+  int okv = 15;
+  int page_v = 0, page_k = -1, page_next = -1;               // pages of V of tile i + 1, K of tile i + 2, and the one after
   if (i0 < i1) {
-    fetch(i0, page);
-    page = page_of(i0 + 1);
-    commit(tiles);
-  }
-  __builtin_amdgcn_s_waitcnt(0x0f70);    // vmcnt(0): q has arrived, said once, or every first product in the loop would wait for the tile on its way
-  for (int i = i0; i < i1; ++i) {
-    char* st = tiles + (TL::NST == 2 ? (i - i0) & 1 : 0) * TL::STAGE;
+    const int p0 = uniform(page_of(i0)), p1 = uniform(page_of(i0 + 1));
+    fetch_k(0, i0, p0);
+    fetch_v(0, i0, p0);
+    if (i0 + 1 < i1) fetch_k(1, i0 + 1, p1);
+    page_next = page_of(i0 + 2);
+    page_v = p1;
+    lds_loads_done();
     __syncthreads();
-    const bool more = i + 1 < i1;
-    if (more) {
-      fetch(i + 1, page);
-      page = page_of(i + 2);
-    }
-    const int j0 = tile_of(i) * 64;
-    // a wave skips tiles that none of its rows sees
-    bool sees = busy && (!a.causal || j0 <= wlast);
-    if (a.window > 0) sees = sees && (j0 + 63 >= wfirst - a.window + 1 || j0 < sinks);
-    if (sees) {
-      const u32x4 okv = *reinterpret_cast<const u32x4*>(st + TL::OK_OFF);
-      // all fragments of 32 tokens are on their way before the first product; the next 32 tokens' replace them one by one
-      f32x16 s[2];
-      Frag kf[KS];
-      const uint32_t st_at = (uint32_t)(uintptr_t)st, k_lane = st_at + k_off<ROWB>(c, sizeof(T) == 2 ? h : 2 * h);
-      uint32_t v_lane = st_at + TL::V_OFF;
-      if constexpr (sizeof(T) == 2) {
-        const int r = lane & 15;
-        v_lane += v_off<ROWB>(4 * h + (r >> 2), 2 * ((lane >> 4) & 1) + ((r & 3) >> 1), T{}) + 8 * (r & 1);
-      }
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[ks] = k_frag32<ROWB>(k_lane, 0, ks, T{});
+    if (busy) {
+      okv = flags(0);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          mma32(s[t], kf[ks], q[ks]);
-          if (t == 0) kf[ks] = k_frag32<ROWB>(k_lane, 1, ks, T{});
-        }
+        for (int ks = 0; ks < KS; ++ks) mma32(s[t], k_frag32<ROWB>(k_lane, t, ks, T{}), q[ks]);
       }
-      Frag vf[NDT];
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);    // vmcnt(0): q has arrived, said once, or every first product in the loop would wait for the tiles on their way
+  for (int i = i0; i < i1; ++i) {
+    const int cur = (i - i0) & 1;
+    lds_loads_done();
+    __syncthreads();                                         // K of tile i + 1 and V of tile i are in place
+    page_k = uniform(page_next);
+    if (i + 2 < i1) fetch_k(cur, i + 2, page_k);
+    if (i + 1 < i1) fetch_v(cur ^ 1, i + 1, page_v);
+    page_v = page_k;
+    page_next = page_of(i + 3);
+    if (busy) {
+      const int j0 = tile_of(i) * 64;
+      const uint32_t kl = k_lane + (cur ^ 1) * TL::TILE, vl = v_lane + cur * TL::TILE;
+      constexpr int RING = sizeof(T) == 2 ? 4 : 1, NX = 4 * NDT;                  // fragments on their way: RING products ahead
+      Frag kf[RING], vf[RING];
 #pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) vf[dt] = v_frag32<ROWB>(v_lane, dt, 0, lane, T{});
-      if constexpr (sizeof(T) == 2) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1 + KS, 0);          // LDS reads
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);             // one product, one read
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
+      for (int x = 0; x < RING; ++x) {
+        kf[x] = k_frag32<ROWB>(kl, x / KS, x % KS, T{});
+        vf[x] = v_frag32<ROWB>(vl, x % NDT, x / NDT, lane, T{});
       }
-      bool inside = uniform(okv[0] & okv[1] & okv[2] & okv[3]) && j0 + 63 <= (a.causal ? wfirst : ti.kv - 1);
+      const int okn = flags(cur ^ 1);
+      bool inside = okv == 15 && j0 + 63 <= (a.causal ? wfirst : ti.kv - 1);
       if (a.window > 0) inside = inside && (j0 >= wlast - a.window + 1 || j0 + 63 < sinks);
       if (!inside) {
 #pragma unroll
@@ -671,7 +677,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int j = j0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-            const bool see = okv[2 * t + (e >> 3)] && j <= see_hi && (j >= see_lo || j < sinks);
+            const bool see = (okv >> (2 * t + (e >> 3)) & 1) & (j <= see_hi) & ((j >= see_lo) | (j < sinks));
             s[t][e] = see ? s[t][e] : -INFINITY;
           }
       }
@@ -698,37 +704,56 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
       }
       const float m_use = m_run == -INFINITY ? 0.f : m_run * cs;
       float psum = 0.f;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      // the probabilities of 16-token step u, rounded to the storage type for the product; their sum is not
+      auto step_p = [&](int u) {
         float pk[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           pk[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + e], cs, -m_use));
           psum += pk[e];
         }
-        // rounded to the storage type for the product; the sum is not
-        const Frag pf = p_frag(pk, T{});
+        return p_frag(pk, T{});
+      };
+      f32x16 sn[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sn[t][e] = 0.f;
+      Frag pf = step_p(0);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        Frag pn = pf;
+        if (u < 3) pn = step_p(u + 1);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-          mma32(ot[dt], vf[dt], pf);
-          if (u < 3) vf[dt] = v_frag32<ROWB>(v_lane, dt, u + 1, lane, T{});
+          const int x = u * NDT + dt;                        // product of the next tile's scores: tokens 32 (x / KS), k step x % KS
+          const int y = x + RING;
+          mma32(sn[x / KS], kf[x % RING], q[x % KS]);
+          if (y < NX) kf[x % RING] = k_frag32<ROWB>(kl, y / KS, y % KS, T{});
+          mma32(ot[dt], vf[x % RING], pf);
+          if (y < NX) vf[x % RING] = v_frag32<ROWB>(vl, y % NDT, y / NDT, lane, T{});
         }
         if constexpr (sizeof(T) == 2) {
-          if (u < 3) {                                       // the next step's exponentials run beside the products
+          if (u < 3) {
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 14 / NDT, 0);
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
               __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-              __builtin_amdgcn_sched_group_barrier(0x002, 28 / NDT, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 14 / NDT, 0);
             }
           }
+        } else {
+          __builtin_amdgcn_sched_barrier(0);                 // or the fragments of all steps are read at once, and spilled
         }
+        pf = pn;
       }
       l_run += psum;
-    }
-    if (more) {
-      if (TL::NST == 1) __syncthreads();
-      commit(tiles + (TL::NST == 2 ? (i + 1 - i0) & 1 : 0) * TL::STAGE);
+      s[0] = sn[0];
+      s[1] = sn[1];
+      okv = okn;
     }
   }
 
