@@ -9,6 +9,7 @@
 //
 // One pass over the keys with a running maximum m and sum l per row (fp32, base-2 exponents):
 //     m' = max(m, max_j s_j),  l' = l 2^(m - m') + sum_j 2^(s_j - m'),  O' = O 2^(m - m') + sum_j 2^(s_j - m') v_j.
+// In bf16 the p_j = 2^(s_j - m') are rounded for the product with v, and l adds up the rounded ones: what is rounded off in the numerator is then missing in the denominator too, and a row that one key dominates loses nothing.
 //
 // A tile is a set of rows of one (request, kv head): `tt` neighbouring rows of the chunk times the gc query heads that
 // share the kv head, so that a key read once serves all of them.  Workgroup t finds its request without any table:
@@ -140,6 +141,21 @@ __device__ __forceinline__ f32x8 p_frag(const float (&x)[8], float) {
     f.hi[i] = x[4 + i];
   }
   return f;
+}
+
+// sum of a fragment's eight elements, as they are stored, on top of l
+__device__ __forceinline__ float add_frag(float l, const bf16x8& f) {
+  const u32x4 u = __builtin_bit_cast(u32x4, f);
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    l += __builtin_bit_cast(float, u[i] << 16);
+    a += __builtin_bit_cast(float, u[i] & 0xffff0000u);
+  }
+  return l + a;
+}
+__device__ __forceinline__ float add_frag(float l, const f32x8& f) {
+  return l + (((f.lo[0] + f.lo[1]) + (f.lo[2] + f.lo[3])) + ((f.hi[0] + f.hi[1]) + (f.hi[2] + f.hi[3])));
 }
 
 // eight elements of a row through a descriptor
@@ -330,15 +346,11 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
     m_run = m_new;
-    float pk[8], psum = 0.f;
+    float pk[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      pk[e] = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - m_use);
-      psum += pk[e];
-    }
-    l_run = l_run * alpha + psum;
-    // the probabilities are rounded to the storage type for the product; their sum is not
+    for (int e = 0; e < 8; ++e) pk[e] = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - m_use);
     const Frag pf = p_frag(pk, T{});
+    l_run = add_frag(l_run * alpha, pf);
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       ot[db] *= alpha;
@@ -703,15 +715,10 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         m_run = m_new;
       }
       const float m_use = m_run == -INFINITY ? 0.f : m_run * cs;
-      float psum = 0.f;
-      // the probabilities of 16-token step u, rounded to the storage type for the product; their sum is not
       auto step_p = [&](int u) {
         float pk[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          pk[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + e], cs, -m_use));
-          psum += pk[e];
-        }
+        for (int e = 0; e < 8; ++e) pk[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + e], cs, -m_use));
         return p_frag(pk, T{});
       };
       f32x16 sn[2];
@@ -733,16 +740,17 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
           mma32(ot[dt], vf[x % RING], pf);
           if (y < NX) vf[x % RING] = v_frag32<ROWB>(vl, y % NDT, y / NDT, lane, T{});
         }
+        l_run = add_frag(l_run, pf);
         if constexpr (sizeof(T) == 2) {
           if (u < 3) {
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
               __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-              __builtin_amdgcn_sched_group_barrier(0x002, 14 / NDT, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 10 / NDT, 0);
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
               __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-              __builtin_amdgcn_sched_group_barrier(0x002, 14 / NDT, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 10 / NDT, 0);
             }
           }
         } else {
@@ -750,7 +758,6 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         }
         pf = pn;
       }
-      l_run += psum;
       s[0] = sn[0];
       s[1] = sn[1];
       okv = okn;
@@ -788,8 +795,65 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   }
 }
 
-// Joins the pieces of a launch's split key axis: a workgroup per (row, head) of its share.  32 threads hold the dims, four
-// each; the eight groups of 32 take every eighth piece, four loads in flight, and meet in LDS.
+// The output row of a (row, head) pair of a launch's workspace; -1 if nothing was written there.
+__device__ __forceinline__ int joined_row(const PageAttnArgs& a, const Split& sp, int wrow) {
+  if (sp.share == 1) {
+    const int b = wrow / sp.per_request, i = wrow - b * sp.per_request;
+    const int c0 = clamp_rows(a.cu_rows[b], a.rows), n = clamp_rows(a.cu_rows[b + 1], a.rows) - c0;
+    return i < n && n <= sp.per_request ? c0 + i : -1;
+  }
+  if (sp.share == 2) {
+    int lo = 0, hi = a.B + 1;                                // the request of this row (B: behind the last one)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu_rows[mid] <= wrow) lo = mid; else hi = mid;
+    }
+    if (lo < a.B && clamp_rows(a.cu_rows[lo + 1], a.rows) - clamp_rows(a.cu_rows[lo], a.rows) <= sp.per_request) return -1;
+  }
+  return wrow;
+}
+
+// Joins few pieces: 32 threads per (row, head), four dims each.  (A workgroup per pair, as below, moved 1 TB/s of the
+// partial results of 80 000 pairs x 3 pieces.)
+constexpr int JOIN_FEW = 32;
+template <typename T>
+__global__ __launch_bounds__(256) void page_attn_join_few_kernel(const PageAttnArgs a, const Split sp) {
+  const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, pieces = sp.pieces, d = lane * 4;
+  if (at >= sp.ws_rows) return;
+  const int wrow = (int)(at / a.heads), head = (int)(at - (long long)wrow * a.heads);
+  const int row = joined_row(a, sp, wrow);
+  if (row < 0) return;
+  float2 p{-INFINITY, 0.f};
+  if (lane < pieces) p = reinterpret_cast<const float2*>(a.ws + sp.ws)[at * pieces + lane];
+  float m = p.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 32));
+  const float f = p.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(p.x - m);     // a piece that saw nothing has no part
+  float l = p.y * f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor(l, o, 32);
+  const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+  const float* src = a.ws + sp.ws + ws_sums(sp.ws_rows, pieces) + at * pieces * a.dim + d;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < pieces; k0 += 4) {
+    f32x4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (k0 + k < pieces && d < a.dim) v[k] = *reinterpret_cast<const f32x4*>(src + (long long)(k0 + k) * a.dim);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = __shfl(f, (k0 + k) & 31, 32);
+      if (k0 + k < pieces) acc += v[k] * w;
+    }
+  }
+  if (d < a.dim) store4(reinterpret_cast<T*>(a.out) + ((long long)row * a.heads + head) * a.dim + d, acc * inv);
+}
+
+// Joins many pieces: a workgroup per (row, head).  32 threads hold the dims, four each; the eight groups of 32 take every
+// eighth piece, four loads in flight, and meet in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs a, const Split sp) {
   __shared__ float s_m[4], s_l[4];
@@ -797,20 +861,8 @@ __global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs 
   __shared__ f32x4 s_acc[8][32];
   const int at = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = sp.pieces;
   const int wrow = at / a.heads, head = at - wrow * a.heads;
-  int row = wrow;
-  if (sp.share == 1) {
-    const int b = wrow / sp.per_request, i = wrow - b * sp.per_request;
-    const int c0 = clamp_rows(a.cu_rows[b], a.rows), n = clamp_rows(a.cu_rows[b + 1], a.rows) - c0;
-    if (i >= n || n > sp.per_request) return;
-    row = c0 + i;
-  } else if (sp.share == 2) {
-    int lo = 0, hi = a.B + 1;                                // the request of this row (B: behind the last one)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu_rows[mid] <= row) lo = mid; else hi = mid;
-    }
-    if (lo < a.B && clamp_rows(a.cu_rows[lo + 1], a.rows) - clamp_rows(a.cu_rows[lo], a.rows) <= sp.per_request) return;
-  }
+  const int row = joined_row(a, sp, wrow);
+  if (row < 0) return;
   float2 p{-INFINITY, 0.f};                                  // MAX_SPLITS pieces: one per thread
   if (tid < pieces) p = reinterpret_cast<const float2*>(a.ws + sp.ws)[(long long)at * pieces + tid];
   float m = p.x;
@@ -941,7 +993,8 @@ int check_args(int dtype, const PageAttnArgs& a) {
 
 template <typename T>
 void join(const PageAttnArgs& a, const Split& s, hipStream_t stream) {
-  if (s.pieces > 1) page_attn_join_kernel<T><<<(unsigned)s.ws_rows, 256, 0, stream>>>(a, s);
+  if (s.pieces > JOIN_FEW) page_attn_join_kernel<T><<<(unsigned)s.ws_rows, 256, 0, stream>>>(a, s);
+  else if (s.pieces > 1) page_attn_join_few_kernel<T><<<(unsigned)((s.ws_rows + 7) / 8), 256, 0, stream>>>(a, s);
 }
 
 template <typename T, int DP>
