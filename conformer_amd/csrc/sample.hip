@@ -18,6 +18,11 @@
 // first histogram leaves in question go to a list in LDS (in index order, a segment per wave): everything above the k-th when
 // top-k is on, so that the rest of the work runs on the list, or the one step that top-p ends in.  A list that does not
 // fit is not made, and the same code runs over the row again.
+//
+// A long row of bf16 logits has few different values (4736 per sign between 2^-30 and 2^7, and 0): there one pass over the
+// row counts every value, the borders and the kept mass follow from the counts times the values' weights, and one more pass
+// adds up the weights, read from a table, in index order.  A value outside that range, if it can matter, sends
+// the row to the general form.
 #include <float.h>
 #include <math.h>
 
@@ -159,6 +164,11 @@ __device__ __forceinline__ double weight(float x, const RowParams& p, const doub
   q = fma(f, q, L);
   q = fma(f, q, 1.0);
   return ldexp(q * table[n & (TABLE - 1)], n >> 8);
+}
+// the same without the table, for few values
+__device__ __forceinline__ double weight_by(float x, const RowParams& p, double unit) {
+  constexpr double L = 0.693147180559945309417 / TABLE;
+  return exp2(fmax(((double)x - (double)p.top) * p.c, -40.0 / L) * (1.0 / TABLE)) * unit;
 }
 __device__ __forceinline__ u64 rounded(double w) { return __builtin_bit_cast(u64, w + MAGIC) & 0xfffffffffffffull; }
 __device__ __forceinline__ u64 units(float x, const RowParams& p, const double* table) { return rounded(weight(x, p, table)); }
@@ -448,7 +458,7 @@ __device__ __forceinline__ Border refine(const SampleLds& lds, const S& s, const
   __syncthreads();
   unsigned base = lds.lo[0], top = lds.lo[1];
   const int log_bins = 31 - __clz(p.nbins);
-  while (top != base) {
+  while (top > base) {                                   // every trip narrows the range to one bin of it
     const int bits = 32 - __clz((int)(top - base));
     const int shift = bits > log_bins ? bits - log_bins : 0;
     clear_bins(lds);
@@ -461,8 +471,8 @@ __device__ __forceinline__ Border refine(const SampleLds& lds, const S& s, const
     });
     at = find_bin(lds, k, target, at.count, at.mass, s.waves);
     base += (unsigned)at.bin << shift;
-    const unsigned end = base + ((1u << shift) - 1);
-    top = end < top ? end : top;
+    const unsigned span = (1u << shift) - 1;                 // base + span may lie behind the last key there is
+    top = top > base && top - base > span ? base + span : top;
   }
   Border b;
   b.key = base;
@@ -555,6 +565,290 @@ __device__ __forceinline__ int by_rank(const SampleLds& lds, const S& s, const R
   return draw(lds, s, p, Limit{value, tie_index(lds, s, value, ties)}, min_p, u);
 }
 
+// ---- rows of bf16 by value ----
+constexpr int BV_LO = (127 - 30) << 7, BV_HI = (127 + 7) << 7;            // bits of 2^-30 and 2^7
+constexpr int BV_SIDE = BV_HI - BV_LO;                                    // values of one sign
+constexpr int BV_ZERO = BV_SIDE, BV_LOW = 2 * BV_SIDE + 1;                // index of 0; of everything at or below -2^7
+constexpr int BV_BINS = BV_LOW + 1;                                       // indices rise with falling value
+constexpr int BV_PER = (BV_BINS + 64 * MAX_WAVES - 1) / (64 * MAX_WAVES);
+constexpr int BV_MIN_VOCAB = 64 * 8 * MAX_WAVES + 1;   // a workgroup of 16 waves; shorter rows would spend their time on the bins
+constexpr int BV_BYTES = BV_PER * 64 * MAX_WAVES * 12 + MAX_WAVES * 12 + 64;
+
+struct ByValueLds {
+  u64* weight;               // [bins], then of the kept values only
+  unsigned* count;           // [bins]
+  u64* part_m;               // [waves]
+  unsigned* part_c;          // [waves]
+  u64* mass;                 // 0: total of the last scan, 1: mass before the border found
+  unsigned* word;            // 0: first bin in use, 1: a row that does not fit, 2: border, 3: count before it, 4: token
+};
+__device__ __forceinline__ ByValueLds carve_by_value(char* p) {
+  ByValueLds l;
+  l.weight = reinterpret_cast<u64*>(p);
+  l.part_m = l.weight + BV_PER * 64 * MAX_WAVES;
+  l.mass = l.part_m + MAX_WAVES;
+  l.count = reinterpret_cast<unsigned*>(l.mass + 2);
+  l.part_c = l.count + BV_PER * 64 * MAX_WAVES;
+  l.word = l.part_c + MAX_WAVES;
+  return l;
+}
+
+__device__ __forceinline__ unsigned bits16(const u32x4& r, int i) { return i & 1 ? r[i >> 1] >> 16 : r[i >> 1] & 0xffffu; }
+// index of a value, not yet kept within the bins: negative for values of 2^7 and more, > BV_LOW for those below -2^7; values
+// between 0 and 2^-30 share the index of 0
+__device__ __forceinline__ int index_of(unsigned u) {
+  const int d = max((int)(u & 0x7fffu) - (BV_LO - 1), 0);
+  return u & 0x8000u ? BV_ZERO + d : BV_ZERO - d;
+}
+__device__ __forceinline__ float value_at(int i) {
+  const int d = i < BV_ZERO ? BV_ZERO - i : i - BV_ZERO;
+  const unsigned u = d == 0 ? 0u : (unsigned)(d + BV_LO - 1) | (i > BV_ZERO ? 0x8000u : 0u);
+  return __builtin_bit_cast(float, u << 16);
+}
+
+// prefix sums over the bins of this thread's first one; lds.mass[0] becomes the whole mass
+__device__ __forceinline__ void before_mine(const ByValueLds& lds, unsigned c, u64 m, int wave, int lane, unsigned& cb, u64& mb) {
+  const unsigned ci = wave_running(c, lane);
+  const u64 mi = wave_running(m, lane);
+  __syncthreads();
+  if (lane == 63) {
+    lds.part_c[wave] = ci;
+    lds.part_m[wave] = mi;
+  }
+  __syncthreads();
+  cb = ci - c;
+  mb = mi - m;
+  u64 total = 0;
+#pragma unroll 4
+  for (int w = 0; w < MAX_WAVES; ++w) {
+    if (w < wave) {
+      cb += lds.part_c[w];
+      mb += lds.part_m[w];
+    }
+    total += lds.part_m[w];
+  }
+  if (wave == 0 && lane == 0) lds.mass[0] = total;
+  __syncthreads();
+}
+
+// false: the row does not fit (for every thread)
+__device__ __forceinline__ bool sample_by_value(char* smem, const RowSource<bf16>& s, float t, int top_k, float top_p, float min_p,
+                                                float u, double unit, int& token) {
+  const ByValueLds lds = carve_by_value(smem);
+  const int tid = threadIdx.x, lane = s.lane, wave = s.wave, n = s.n;
+#pragma unroll
+  for (int j = 0; j < BV_PER; ++j) lds.count[j * 64 * MAX_WAVES + tid] = 0;
+  if (tid == 0) {
+    lds.word[0] = BV_BINS;
+    lds.word[1] = 0;
+    lds.word[2] = BV_LOW;
+  }
+  __syncthreads();
+  // ---- one pass: count every value ----
+  {
+    int least = 0;
+    bool odd = false;
+    s.vectors(0, n, [&](int e, const u32x4& raw) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const unsigned v = bits16(raw, k);
+        const int i = index_of(v);
+        least = min(least, i);
+        odd |= (v & 0x7fffu) - 1u < (unsigned)BV_LO - 1u;                 // between 0 and 2^-30
+        atomicAdd(&lds.count[min(max(i, 0), BV_LOW)], 1u);                // -inf and NaN among the low ones, and what fills up the row
+      }
+    });
+    if (least < 0 || odd) lds.word[1] = 1;
+  }
+  __syncthreads();
+  unsigned cnt[BV_PER];
+  int first = BV_BINS;
+#pragma unroll
+  for (int j = BV_PER - 1; j >= 0; --j) {
+    const int i = tid * BV_PER + j;
+    cnt[j] = i < BV_LOW ? lds.count[i] : 0;
+    first = cnt[j] ? i : first;
+  }
+  if (first < BV_BINS) atomicMin(&lds.word[0], (unsigned)first);
+  __syncthreads();
+  const int top_i = (int)lds.word[0];
+  if (lds.word[1] || top_i >= BV_LOW) return false;
+  const float top = value_at(top_i);
+  if ((double)top + 128.0 < 40.0 * (double)t ? lds.count[BV_LOW] > 0 : false) return false;      // low values that weigh something
+  RowParams p;
+  p.top = top;
+  p.bins = 0.f;
+  p.nbins = 0;
+  p.c = TABLE / 0.693147180559945309417 / (double)t;
+
+  // ---- weights, and the borders ----
+  unsigned c = 0;
+  u64 m = 0, w[BV_PER];
+#pragma unroll
+  for (int j = 0; j < BV_PER; ++j) {
+    const int i = tid * BV_PER + j;
+    w[j] = cnt[j] ? rounded(weight_by(value_at(i), p, unit)) : 0;
+    c += cnt[j];
+    m += cnt[j] * w[j];
+  }
+  unsigned cb;
+  u64 mb;
+  before_mine(lds, c, m, wave, lane, cb, mb);
+  int border = BV_LOW;                                       // the last value kept, how many of it, and the mass before it
+  unsigned ties = 0;
+  u64 before = lds.mass[0], total = before;
+  auto publish = [&](int j, unsigned count_before, u64 mass_before) {
+    lds.word[2] = (unsigned)(tid * BV_PER + j);
+    lds.word[3] = count_before;
+    lds.mass[1] = mass_before;
+    lds.part_m[0] = w[j];
+  };
+  if (top_k > 0 && top_k < n) {
+    unsigned cc = cb;
+    u64 mm = mb;
+#pragma unroll
+    for (int j = 0; j < BV_PER; ++j) {
+      if (cc < (unsigned)top_k && (unsigned)top_k <= cc + cnt[j]) publish(j, cc, mm);
+      cc += cnt[j];
+      mm += cnt[j] * w[j];
+    }
+    __syncthreads();
+    if (lds.word[2] != BV_LOW) {                             // else k reaches the low values: all others are kept
+      border = (int)lds.word[2];
+      ties = (unsigned)top_k - lds.word[3];
+      before = lds.mass[1];
+      total = before + ties * lds.part_m[0];
+    }
+    __syncthreads();
+  }
+  if (top_p < 1.f) {
+    const double target = (double)top_p * (double)total;
+    u64 mm = mb;
+#pragma unroll
+    for (int j = 0; j < BV_PER; ++j) {
+      if ((double)mm < target && target <= (double)(mm + cnt[j] * w[j])) publish(j, 0, mm);
+      mm += cnt[j] * w[j];
+    }
+    __syncthreads();
+    const double r = ceil((target - (double)lds.mass[1]) / (double)lds.part_m[0]);      // kept while mass + i w < target
+    const unsigned rr = r < 1.0 ? 1u : (r > (double)MAX_VOCAB ? (unsigned)MAX_VOCAB : (unsigned)r);
+    const int at = (int)lds.word[2];
+    ties = at == border && rr > ties ? ties : rr;
+    border = at;
+    before = lds.mass[1];
+    total = before + ties * lds.part_m[0];
+    __syncthreads();
+  }
+  if (min_p > 0.f) {                                         // values whose weight is below min_p fall away whole
+    const double least = (double)top + log((double)fminf(min_p, 1.f)) * (double)t;
+    u64 cut = 0;
+    int last = -1;
+#pragma unroll
+    for (int j = 0; j < BV_PER; ++j) {
+      const int i = tid * BV_PER + j;
+      if (i < border && cnt[j] && ((double)value_at(i) >= least || i == top_i)) {
+        cut += cnt[j] * w[j];
+        last = i;
+      }
+    }
+    const bool whole = border < BV_LOW && ((double)value_at(border) >= least || border == top_i);
+    cut = wave_total(cut);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o));
+    if (lane == 0) {
+      lds.part_m[wave] = cut;
+      lds.part_c[wave] = (unsigned)(last + 1);
+    }
+    __syncthreads();
+    if (!whole) {                                            // every kept value lies before the border, with all its tokens
+      before = 0;
+      int end = 0;
+      for (int k = 0; k < MAX_WAVES; ++k) {
+        before += lds.part_m[k];
+        end = max(end, (int)lds.part_c[k]);
+      }
+      border = end;
+      ties = 0;
+      total = before;
+    }
+    __syncthreads();
+  }
+
+  // ---- the draw: weights of the kept values by index, the border's apart ----
+  const bool zero = !(u > 0.f);                              // u = 0 (or NaN): the first kept token whose weight is a number at all
+#pragma unroll
+  for (int j = 0; j < BV_PER; ++j) {
+    const int i = tid * BV_PER + j;
+    if (zero && cnt[j]) w[j] = ((double)value_at(i) - (double)top) * p.c > -745.13 * (TABLE / 0.693147180559945309417);
+    lds.weight[i] = i < border ? w[j] : 0;
+    if (i == border) lds.mass[1] = w[j];
+  }
+  __syncthreads();
+  const u64 w_border = ties > 0 ? lds.mass[1] : 0;
+  u64 target = 0;
+  if (!zero) {
+    target = (u64)((double)(u < 1.f ? u : 0.99999994f) * (double)total);
+    target = target < total ? target : total - 1;
+  }
+  int from = 0, to = n;
+  for (int level = 0; level < 2; ++level) {
+    u64 sum = 0;
+    unsigned eq = 0;
+    s.vectors(from, to, [&](int e, const u32x4& raw) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = min(index_of(bits16(raw, k)), BV_LOW);
+        sum += lds.weight[i];
+        eq += i == border;
+      }
+    });
+    sum = wave_total(sum);
+    eq = wave_total(eq);
+    __syncthreads();
+    if (lane == 0) {
+      lds.part_m[wave] = sum;
+      lds.part_c[wave] = eq;
+    }
+    __syncthreads();
+    int k = 0;
+    for (; k < MAX_WAVES; ++k) {                             // the wave's piece in which the running sum passes the target
+      const unsigned e = min(lds.part_c[k], ties);
+      const u64 piece_sum = lds.part_m[k] + e * w_border;
+      if (piece_sum > target || k == MAX_WAVES - 1) break;
+      target -= piece_sum;
+      ties -= e;
+    }
+    const int step = s.piece(from, to);
+    from += k * step;
+    to = from + step < to ? from + step : to;
+  }
+  if (wave == 0) {
+    int at = -1;
+    for (int e0 = from; e0 < to && at < 0; e0 += 512) {
+      const int e = e0 + 8 * lane;
+      const u32x4 raw = load_raw(s.row, e < to ? e : n, n);
+      u64 v[8];
+      unsigned eq = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) eq += min(index_of(bits16(raw, k)), BV_LOW) == border;
+      unsigned rank = wave_running(eq, lane) - eq;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = min(index_of(bits16(raw, k)), BV_LOW);
+        v[k] = i == border ? (rank++ < ties ? w_border : 0) : lds.weight[i];
+      }
+      const unsigned here = wave_total(eq);
+      at = pick_in_wave(v, lane, target);
+      if (at >= 0) at += e0;
+      ties -= min(here, ties);
+    }
+    if (lane == 0) lds.word[4] = (unsigned)at;
+  }
+  __syncthreads();
+  token = (int)lds.word[4];
+  return true;
+}
+
 template <typename T>
 __global__ __launch_bounds__(64 * MAX_WAVES) void sample_kernel(const SampleArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -564,6 +858,21 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void sample_kernel(const SampleArgs
   const RowSource<T> s{reinterpret_cast<const T*>(a.logits) + (long long)r * a.row_stride, n, wave, waves, lane};
   const int log_n = n > 1 ? 32 - __clz(n - 1) : 0;
   const double unit = ldexp(1.0, log_n > 12 ? 63 - log_n : 51);
+  const float t = a.temperature ? a.temperature[r] : 1.f;
+  const int top_k = a.top_k ? a.top_k[r] : 0;
+  const float top_p = a.top_p ? a.top_p[r] : 1.f;
+  const float min_p = a.min_p ? a.min_p[r] : 0.f;
+  const bool greedy = !(t > 0.f) || top_k == 1 || top_p <= 0.f;
+  int token;
+  if constexpr (sizeof(T) == 2) {
+    if (n >= BV_MIN_VOCAB && !greedy) {
+      if (sample_by_value(smem, s, t, top_k, top_p, min_p, a.u[r], unit, token)) {
+        if (tid == 0) a.tokens[r] = token;
+        return;
+      }
+      __syncthreads();
+    }
+  }
   for (int i = tid; i < TABLE; i += blockDim.x) lds.table[i] = exp_table.v[i] * unit;
 
   // the largest logit, and the lane's first vector that holds its own largest
@@ -584,14 +893,9 @@ __global__ __launch_bounds__(64 * MAX_WAVES) void sample_kernel(const SampleArgs
   for (int w = 0; w < waves; ++w) top = fmaxf(top, __builtin_bit_cast(float, lds.part_c[w]));
   __syncthreads();
 
-  const float t = a.temperature ? a.temperature[r] : 1.f;
-  const int top_k = a.top_k ? a.top_k[r] : 0;
-  const float top_p = a.top_p ? a.top_p[r] : 1.f;
-  const float min_p = a.min_p ? a.min_p[r] : 0.f;
-  int token;
   if (top == -INFINITY) {
     token = -1;
-  } else if (!(t > 0.f) || top_k == 1 || top_p <= 0.f) {
+  } else if (greedy) {
     if (tid == 0) lds.lo[0] = 0xffffffffu;
     __syncthreads();
     if (lane_top == top) atomicMin(&lds.lo[0], (unsigned)top_at);
@@ -651,8 +955,9 @@ int launch_sample_tokens(int dtype, const SampleArgs& a, hipStream_t stream) {
   int waves = 1;
   while (waves < MAX_WAVES && waves * 512 < a.vocab) waves *= 2;
   auto k = dtype == DT_BF16 ? sample_kernel<bf16> : sample_kernel<float>;
-  if (reserve_lds(reinterpret_cast<const void*>(k), lds_bytes(MAX_WAVES)) != hipSuccess) return fail("sample_tokens: cannot reserve %d bytes of LDS", lds_bytes(MAX_WAVES));
-  k<<<a.rows, 64 * waves, lds_bytes(waves), stream>>>(a);
+  const int bytes = dtype == DT_BF16 && a.vocab >= BV_MIN_VOCAB && BV_BYTES > lds_bytes(waves) ? BV_BYTES : lds_bytes(waves);
+  if (reserve_lds(reinterpret_cast<const void*>(k), bytes) != hipSuccess) return fail("sample_tokens: cannot reserve %d bytes of LDS", bytes);
+  k<<<a.rows, 64 * waves, bytes, stream>>>(a);
   return check_launch("sample_tokens");
 }
 

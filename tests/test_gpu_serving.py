@@ -321,6 +321,42 @@ def test_sampling_masked_and_non_finite_logits():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [8, 64, 700, 9001])
+def test_sampling_when_top_k_reaches_masked_tokens(dtype, v):
+    """Tokens masked with the type's lowest value or -inf, fewer others than k: the border lies at the far end of the keys
+    (a range of keys that ends at the last one there is)."""
+    g = torch.Generator().manual_seed(v)
+    for fill in (torch.finfo(dtype).min, -math.inf, -1e4):
+        for t in (0.1, 1.0):
+            x = (torch.randn(6, v, generator=g) * 2.2).to(dtype)
+            x[torch.rand(6, v, generator=g) < 0.4] = fill
+            x[:, 0] = 1.0
+            u, k = torch.rand(6, generator=g).tolist(), [max(1, v * 4 // 5)] * 6
+            for m in (None, [0.01] * 6):
+                assert _sample(x, u, [t] * 6, k, None, m) == _want(x, u, [t] * 6, k, None, m), (fill, t, m)
+
+
+@pytest.mark.parametrize("v", [8192, 8193, 12345])
+def test_sampling_long_bf16_rows_at_the_ends_of_the_value_range(v):
+    """Values around 2^-30 and 2^7, zeros of both signs, large temperatures that give low values weight, filters that end
+    inside equal values."""
+    g = torch.Generator().manual_seed(v)
+    r = 8
+    u = torch.rand(r, generator=g).tolist()
+    u[0] = 0.0
+    rows = {"tiny": torch.randn(r, v, generator=g) * 2.0 ** -30, "huge": torch.randn(r, v, generator=g) * 60,
+            "zeros": torch.where(torch.rand(r, v, generator=g) < 0.5, -0.0, 0.0), "below": -130 - torch.rand(r, v, generator=g),
+            "low": torch.where(torch.rand(r, v, generator=g) < 0.3, -200.0, torch.randn(r, v, generator=g)),
+            "edge": torch.tensor([127.5, -127.5, 2.0 ** -30, -2.0 ** -30, 0.0, 1.0, -1.0])[torch.randint(0, 7, (r, v), generator=g)],
+            "steps": (torch.randn(r, v, generator=g) * 3).round()}
+    for name, x in rows.items():
+        x = x.bfloat16()
+        for t, k, p, m in ((None, None, None, None), ([9.0] * r, None, [0.7] * r, None), (None, [v // 3] * r, [0.6] * r, [0.1] * r),
+                           ([1.5] * r, [v - 1] * r, None, [1.0] * r), (None, None, [0.5, 0.05] * (r // 2), None)):
+            assert _sample(x, u, t, k, p, m) == _want(x, u, t, k, p, m), (name, t, k, p, m)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_sampling_where_one_step_of_the_histogram_holds_too_many(dtype):
     """Thousands of equal logits, and thousands within one step: the candidate list does not fit."""
     n = 1 << 15
