@@ -656,7 +656,7 @@ def _on(t: Tensor, device: torch.device, dtype: torch.dtype, name: str, ndim: in
         raise TypeError(f"fcenc: {name} must be {dtype}, got {t.dtype}")
     if t.dim() != ndim:
         raise ValueError(f"fcenc: {name} must have {ndim} dims, got {tuple(t.shape)}")
-    if t.numel() > 1 and t.stride(-1) != 1 and t.shape[-1] > 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"fcenc: {name} must be contiguous along its last dimension")
     return t
 
@@ -714,8 +714,7 @@ def kv_page_plan_(kv_lens: Tensor, new_lens: Tensor, finished: Optional[Tensor],
     _launch(dev, N.lib().fcenc_page_plan, kv_lens.data_ptr(), new_lens.data_ptr(), N.ptr(finished), b, block_table.data_ptr(),
             block_table.stride(0) if b > 1 else w, w, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size,
             slots.data_ptr(), rows, cu_rows.data_ptr(), granted.data_ptr())
-    for t in (kv_lens, block_table, free_pages, free_count):
-        torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version((kv_lens, block_table, free_pages, free_count))
     return slots, cu_rows, granted
 
 
@@ -745,8 +744,7 @@ def kv_page_write_(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots
     ks, vs = k.stride(), v.stride()
     _launch(dev, N.lib().fcenc_page_write, _cdt(k), C.byref(pages), k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1],
             slots.data_ptr(), n)
-    torch.autograd.graph.increment_version(k_pages)
-    torch.autograd.graph.increment_version(v_pages)
+    torch.autograd.graph.increment_version((k_pages, v_pages))
 
 
 @_fake(kv_page_write_)
