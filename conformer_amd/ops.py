@@ -648,33 +648,33 @@ def _no_grad(*operands: Tensor) -> None:
         raise RuntimeError("fcenc: the serving operators have no backward pass; call them under torch.no_grad()")
 
 
-def _on(t: Tensor, device: torch.device, dtype: torch.dtype, name: str, ndim: int) -> Tensor:
-    """An operand of the serving operators: on `device`, unit stride along its last dimension."""
-    if t.device != device or not t.is_cuda:
-        raise RuntimeError(f"fcenc: {name} must live on the GPU, beside the other operands (got {t.device}, {device})")
+def _on(t: Tensor, dev: int, dtype: torch.dtype, name: str, ndim: int) -> None:
+    """An operand of the serving operators: on GPU `dev`, unit stride along its last dimension."""
+    if t.get_device() == dev >= 0 and t.dtype is dtype and t.dim() == ndim and (t.stride(-1) == 1 or t.shape[-1] <= 1):
+        return
+    if t.get_device() != dev or dev < 0:
+        raise RuntimeError(f"fcenc: {name} must live on the GPU, beside the other operands (got {t.device})")
     if t.dtype != dtype:
         raise TypeError(f"fcenc: {name} must be {dtype}, got {t.dtype}")
     if t.dim() != ndim:
         raise ValueError(f"fcenc: {name} must have {ndim} dims, got {tuple(t.shape)}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"fcenc: {name} must be contiguous along its last dimension")
-    return t
+    raise ValueError(f"fcenc: {name} must be contiguous along its last dimension")
 
 
-def _launch(device: torch.device, call, *args) -> None:
-    """call(*args, the device's current stream) with `device` current: a kernel is launched on the device that is,
+def _launch(dev: int, call, *args) -> None:
+    """call(*args, the GPU's current stream) with GPU `dev` current: a kernel is launched on the device that is,
     whatever its stream belongs to."""
-    stream = torch._C._cuda_getCurrentRawStream(device.index)
-    if device.index == torch.cuda.current_device():
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
         rc = call(*args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(dev):
             rc = call(*args, stream)
     if rc != 0:
         N.check(rc)
 
 
-def _pages(k_pages: Tensor, v_pages: Tensor, dev: torch.device, dt: torch.dtype) -> N.Pages:
+def _pages(k_pages: Tensor, v_pages: Tensor, dev: int, dt: torch.dtype) -> N.Pages:
     _on(k_pages, dev, dt, "k_pages", 4)
     _on(v_pages, dev, dt, "v_pages", 4)
     n, h, ps, d = k_pages.shape
@@ -693,7 +693,7 @@ def kv_page_plan_(kv_lens: Tensor, new_lens: Tensor, finished: Optional[Tensor],
     (slots int64 [rows], cu_rows int32 [B + 1], granted bool [B]).  A row is granted when its tokens fit the table and the step's
     rows and it needs no page, or the stack covers all that rows 0 .. b want: its pages move from the stack to the table and
     kv_lens grows.  Slots are page * page_size + offset; -1 for refused requests and rows that belong to nobody."""
-    dev = kv_lens.device
+    dev = kv_lens.get_device()
     _on(kv_lens, dev, torch.int32, "kv_lens", 1)
     _on(new_lens, dev, torch.int32, "new_lens", 1)
     _on(block_table, dev, torch.int32, "block_table", 2)
@@ -708,9 +708,9 @@ def kv_page_plan_(kv_lens: Tensor, new_lens: Tensor, finished: Optional[Tensor],
             raise ValueError("fcenc::kv_page_plan_: finished must hold one entry per table row")
     if rows < 0 or rows >= 2 ** 31 or b == 0 or w == 0 or free_pages.numel() == 0:
         raise ValueError(f"fcenc::kv_page_plan_: {rows} rows, table {b} x {w}, {free_pages.numel()} pages")
-    slots = torch.empty((rows,), dtype=torch.int64, device=dev)
-    cu_rows = torch.empty((b + 1,), dtype=torch.int32, device=dev)
-    granted = torch.empty((b,), dtype=torch.bool, device=dev)
+    slots = torch.empty(rows, dtype=torch.int64, device=kv_lens.device)
+    cu_rows = torch.empty(b + 1, dtype=torch.int32, device=kv_lens.device)
+    granted = torch.empty(b, dtype=torch.bool, device=kv_lens.device)
     _launch(dev, N.lib().fcenc_page_plan, kv_lens.data_ptr(), new_lens.data_ptr(), N.ptr(finished), b, block_table.data_ptr(),
             block_table.stride(0) if b > 1 else w, w, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size,
             slots.data_ptr(), rows, cu_rows.data_ptr(), granted.data_ptr())
@@ -730,7 +730,7 @@ def kv_page_write_(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots
     """Rows of k and v [N][Hkv][D] (strided views of a fused projection are fine) into pages [P][Hkv][page_size][D] at
     slots int64 [N]; a slot outside the pool (-1) is skipped.  Slots must differ: of two rows with one slot either may
     stay."""
-    dev = k_pages.device
+    dev = k_pages.get_device()
     _no_grad(k, v, k_pages, v_pages)
     _on(k, dev, k_pages.dtype, "k", 3)
     _on(v, dev, k_pages.dtype, "v", 3)
@@ -760,7 +760,7 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
     kv_lens int32 [B] -> [N][H][D].  The row at position p = kv_lens[b] - n + i sees token j < kv_lens[b] if
     (not causal or j <= p) and (window == 0 or j > p - window or j < sinks).  Rows that see nothing, or belong to no request,
     are zeros.  `max_rows` = the longest chunk, if the caller knows it (0: unknown): a hint for speed only."""
-    dev = q.device
+    dev = q.get_device()
     _no_grad(q, k_pages, v_pages)
     _on(q, dev, q.dtype, "q", 3)
     pages = _pages(k_pages, v_pages, dev, q.dtype)
@@ -773,14 +773,14 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
         raise ValueError(f"fcenc::kv_page_attention: q {tuple(q.shape)}, pages {tuple(k_pages.shape)}, {b} table rows, "
                          f"{kv_lens.numel()} lengths, {cu_rows.numel()} row offsets")
     dt = _cdt(q)
-    out = torch.empty((n, h, d), dtype=q.dtype, device=dev)
+    out = torch.empty(n, h, d, dtype=q.dtype, device=q.device)
     if n == 0:
         return out
     rows = N.PageRows(q.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_rows.data_ptr(), q.stride(0), q.stride(1),
                       block_table.stride(0) if b > 1 else w, b, n, h, w, window, sinks, int(causal), max_rows, scale)
     lib = N.lib()
     need = lib.fcenc_page_attention_workspace_bytes(dt, C.byref(pages), C.byref(rows))
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _launch(dev, lib.fcenc_page_attention, dt, C.byref(pages), C.byref(rows), out.data_ptr(), N.ptr(ws), need)
     return out
 
@@ -799,19 +799,18 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Optional[Tensor] = Non
     (>= 1: all), min_p fp32 [R] those of at least min_p times the largest weight (<= 0: all); the first is always kept.
     The token is the first one, in index order, whose running mass exceeds u times the kept mass.  temperature <= 0
     takes the first maximum.  NaN logits count as -inf; a row without any other gives -1."""
-    dev = logits.device
+    dev = logits.get_device()
     _no_grad(logits)
     _on(logits, dev, logits.dtype, "logits", 2)
     r, v = logits.shape
-    for nm, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                      ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+    for nm, t in (("u", u), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
         if t is not None:
-            _on(t, dev, dt, nm, 1)
+            _on(t, dev, torch.int32 if nm == "top_k" else torch.float32, nm, 1)
             if t.numel() != r:
                 raise ValueError(f"fcenc::sample_tokens: {nm} must hold one value per row")
     if v == 0:
         raise ValueError("fcenc::sample_tokens: empty vocabulary")
-    tokens = torch.empty((r,), dtype=torch.int32, device=dev)
+    tokens = torch.empty(r, dtype=torch.int32, device=logits.device)
     if r == 0:
         return tokens
     _launch(dev, N.lib().fcenc_sample_tokens, _cdt(logits), logits.data_ptr(), logits.stride(0) if r > 1 else v, r, v,
