@@ -831,6 +831,8 @@ int fcenc_page_plan(int32_t* kv_lens, const int32_t* new_lens, const uint8_t* fi
   return launch_page_plan(a, (hipStream_t)stream);
 }
 
+// the stride of a dimension of one element means nothing
+static long long stride_of(long long stride, int size, int es) { return size > 1 ? stride * es : 0; }
 static int element_bytes(int dtype) { return dtype == FCENC_BF16 ? 2 : dtype == FCENC_F32 ? 4 : 0; }
 
 int fcenc_page_write(int dtype, const fcenc_pages* pages, const void* k, const void* v, long long k_row, long long k_head,
@@ -840,9 +842,11 @@ int fcenc_page_write(int dtype, const fcenc_pages* pages, const void* k, const v
   if (!pages) return fail("page_write: null pages");
   PageWriteArgs a;
   a.k = (const char*)k; a.v = (const char*)v; a.k_pages = (char*)pages->k; a.v_pages = (char*)pages->v; a.slots = slots;
-  a.k_row = k_row * es; a.k_head = k_head * es; a.v_row = v_row * es; a.v_head = v_head * es;
-  a.k_page = pages->k_page * es; a.k_phead = pages->k_head * es; a.k_slot = pages->k_slot * es;
-  a.v_page = pages->v_page * es; a.v_phead = pages->v_head * es; a.v_slot = pages->v_slot * es;
+  a.k_row = stride_of(k_row, rows, es); a.k_head = stride_of(k_head, pages->kv_heads, es);
+  a.v_row = stride_of(v_row, rows, es); a.v_head = stride_of(v_head, pages->kv_heads, es);
+  a.k_page = stride_of(pages->k_page, pages->n_pages, es); a.k_phead = stride_of(pages->k_head, pages->kv_heads, es);
+  a.v_page = stride_of(pages->v_page, pages->n_pages, es); a.v_phead = stride_of(pages->v_head, pages->kv_heads, es);
+  a.k_slot = pages->k_slot * es; a.v_slot = pages->v_slot * es;
   a.rows = rows; a.heads = pages->kv_heads; a.head_bytes = pages->head_dim * es; a.n_pages = pages->n_pages;
   a.shift = page_shift(pages->page_size);
   return launch_page_write(a, (hipStream_t)stream);
@@ -856,12 +860,14 @@ static int page_attn_args(int dtype, const fcenc_pages* p, const fcenc_page_rows
   if (p->k_slot < 0 || p->v_slot < 0 || p->k_slot * es > slot_max || p->v_slot * es > slot_max) return fail("page_attention: slot strides %lld / %lld", p->k_slot, p->v_slot);
   a.q = (const char*)r->q; a.k = (const char*)p->k; a.v = (const char*)p->v;
   a.table = r->block_table; a.kv_lens = r->kv_lens; a.cu_rows = r->cu_rows;
-  a.q_row = r->q_row * es; a.q_head = r->q_head * es;
-  a.k_page = p->k_page * es; a.k_head = p->k_head * es; a.k_slot = (int)(p->k_slot * es);
-  a.v_page = p->v_page * es; a.v_head = p->v_head * es; a.v_slot = (int)(p->v_slot * es);
+  a.q_row = stride_of(r->q_row, r->rows, es); a.q_head = stride_of(r->q_head, r->heads, es);
+  a.k_page = stride_of(p->k_page, p->n_pages, es); a.k_head = stride_of(p->k_head, p->kv_heads, es); a.k_slot = (int)(p->k_slot * es);
+  a.v_page = stride_of(p->v_page, p->n_pages, es); a.v_head = stride_of(p->v_head, p->kv_heads, es); a.v_slot = (int)(p->v_slot * es);
   a.table_row = r->table_row; a.width = r->table_width; a.B = r->batch; a.rows = r->rows; a.heads = r->heads;
   a.kv_heads = p->kv_heads; a.dim = p->head_dim; a.n_pages = p->n_pages; a.shift = page_shift(p->page_size);
-  a.window = r->window; a.sinks = r->sinks; a.causal = r->causal; a.max_rows = r->max_rows; a.scale = r->scale;
+  // a window as long as the table is none (and positions minus window stay within 32 bits)
+  a.window = r->window > 0 && r->window >= ((long long)r->table_width << (a.shift > 0 ? a.shift : 0)) ? 0 : r->window;
+  a.sinks = r->sinks; a.causal = r->causal; a.max_rows = r->max_rows; a.scale = r->scale;
   return 0;
 }
 

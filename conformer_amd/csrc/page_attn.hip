@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   const int last = first + (ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt) - 1;
   int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
   if (ti.b == a.B || hi < 0) hi = 0;
-  int lo = a.window > 0 ? first - a.window + 1 : 0;
+  int lo = a.window > 0 && first > 0 ? first - a.window + 1 : 0;
   lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
   const int sinks = a.window > 0 ? a.sinks : 0;
   const int lob = lo >> 5;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   const bool live = rt < tt && ti.t0 + rt < ti.n && rh < group;
   const int pos = first + rt;
   const int see_hi = a.causal ? pos : ti.kv - 1;             // last token it sees
-  const int see_lo = a.window > 0 ? pos - a.window + 1 : 0;  // first one, next to the sinks
+  const int see_lo = a.window > 0 && pos > 0 ? pos - a.window + 1 : 0;  // first one, next to the sinks
   Frag q[KS];
   {
     const char* qrow = a.q + (long long)(ti.c0 + ti.t0 + (live ? rt : 0)) * a.q_row + (long long)(kvh * group + (live ? rh : 0)) * a.q_head;
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   const int last = first + live_tt - 1;
   int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
   if (ti.b == a.B || hi < 0) hi = 0;
-  int lo = a.window > 0 ? first - a.window + 1 : 0;
+  int lo = a.window > 0 && first > 0 ? first - a.window + 1 : 0;
   lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
   const int sinks = a.window > 0 ? a.sinks : 0;
   const int lot = lo >> 6;
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   const bool live = rt < live_tt && rh < group;
   const int pos = first + rt;
   const int see_hi = a.causal ? pos : ti.kv - 1;
-  const int see_lo = a.window > 0 ? pos - a.window + 1 : 0;
+  const int see_lo = a.window > 0 && pos > 0 ? pos - a.window + 1 : 0;
   const int wt0 = (32 * wave) / gc;
   int wt1 = (32 * wave + 31) / gc;
   wt1 = wt1 < live_tt - 1 ? wt1 : live_tt - 1;

@@ -759,7 +759,9 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
     (rows cu_rows[b] .. cu_rows[b+1] - 1 belong to request b), pages [P][Hkv][page_size][D], block_table int32 [B][W],
     kv_lens int32 [B] -> [N][H][D].  The row at position p = kv_lens[b] - n + i sees token j < kv_lens[b] if
     (not causal or j <= p) and (window == 0 or j > p - window or j < sinks).  Rows that see nothing, or belong to no request,
-    are zeros.  `max_rows` = the longest chunk, if the caller knows it (0: unknown): a hint for speed only."""
+    are zeros.  Slots that no row of a chunk sees may hold anything; a NaN or infinity among the values (V) that some row sees
+    may also reach rows of the same chunk that do not.  `max_rows` = the longest chunk, if the caller knows it (0: unknown): a
+    hint for speed only."""
     dev = q.get_device()
     _no_grad(q, k_pages, v_pages)
     _on(q, dev, q.dtype, "q", 3)

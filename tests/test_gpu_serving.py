@@ -110,6 +110,26 @@ def test_attention_hint_changes_nothing_but_speed(max_rows):
     _check(got, q, kp, vp, table, kv, cu, 0.2, torch.bfloat16)
 
 
+def test_attention_extreme_windows_and_unit_dimensions():
+    """A window of 2^31 - 1 tokens is none, also where rows in front of the request's start share a tile with others; strides of
+    dimensions of one element are not looked at."""
+    new, kv = [7, 50], [3, 41]
+    q, kp, vp, table, cu = _problem(torch.bfloat16, 2, 1, 64, 16, new, kv, 19)
+    want = _run(q, kp, vp, table, kv, cu, 0.125)
+    for causal in (True, False):
+        got = _run(q, kp, vp, table, kv, cu, 0.125, window=2 ** 31 - 1, sinks=2 ** 31 - 1, causal=causal)
+        _check(got, q, kp, vp, table, kv, cu, 0.125, torch.bfloat16, causal=causal)
+        assert torch.equal(got, want) or not causal
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    odd = lambda t: t.cuda().as_strided(t.shape, (t.stride(0), 3, t.stride(2), 1))           # one kv head
+    one = q[:1, :1].cuda().as_strided((1, 1, 64), (5, 7, 1))                                   # one row, one head
+    got = ops.kv_page_attention(one, odd(kp), odd(vp), i32(table[1:]), i32([41]), i32([0, 1]), 0.125)
+    _check(got, q[:1, :1], kp, vp, table[1:], [41], [0, 1], 0.125, torch.bfloat16)
+    k = torch.randn(1, 1, 64).bfloat16().cuda()
+    kc, vc = kp.cuda(), vp.cuda()
+    ops.kv_page_write_(k.as_strided((1, 1, 64), (1, 1, 1)), k, odd(kc), odd(vc), torch.tensor([16 * table[0][0] + 5]).cuda())
+
+
 @pytest.mark.parametrize("many", [70, 300, 4200])
 def test_attention_many_requests(many):
     """The search for a tile's request over more than 64 and more than 4096 of them, with empty ones among them."""
