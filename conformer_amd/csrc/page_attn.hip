@@ -431,8 +431,7 @@ struct ChunkTile {
   static constexpr int KT = 64;                                  // tokens of a tile
   static constexpr int TILE = KT * ROWB;
   static constexpr int V_OFF = 2 * TILE;                         // two K tiles, two V tiles; all at multiples of 256: see lds_at
-  static constexpr int OK_OFF = 4 * TILE;                        // 2 x 4 flags: the page of every 16 tokens exists
-  static constexpr int BYTES = OK_OFF + 32;
+  static constexpr int BYTES = 4 * TILE;
 };
 
 // Where 16-byte piece `ch` of row `row` lies, so that reads spread over the 256 bytes of the 64 LDS banks.  K: 16 rows that are
@@ -506,16 +505,64 @@ __device__ __forceinline__ void lds_load16(uint32_t dst, const char* base, uint3
 __device__ __forceinline__ void lds_load16(uint32_t dst, const char* src) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
 }
+// N of them, to `dst` + 1024 v.  The offset in the instruction counts for both addresses (and reaches 4095), so load v's
+// `off` is what its 16 bytes are away from base + 1024 (v % 4).
+template <int N>
+__device__ __forceinline__ void lds_loads(uint32_t dst, const char* base, const uint32_t (&off)[N]) {
+  static_assert(N == 2 || N % 4 == 0, "pairs or fours");
+  if constexpr (N == 2) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 1\n\t"
+        "global_load_lds_dwordx4 %1, %3\n\t"
+        "global_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(dst), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
+  } else {
+#pragma unroll
+    for (int v = 0; v < N; v += 4)
+      asm volatile(
+          "s_mov_b32 m0, %0\n\ts_nop 1\n\t"
+          "global_load_lds_dwordx4 %1, %5\n\t"
+          "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
+          "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
+          "global_load_lds_dwordx4 %4, %5 offset:3072"
+          ::"s"(dst + v * 1024), "v"(off[v]), "v"(off[v + 1]), "v"(off[v + 2]), "v"(off[v + 3]), "s"(base) : "memory");
+  }
+}
 __device__ __forceinline__ void lds_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ const u32x4 zero16 = {0, 0, 0, 0};
 
-template <typename T, int DP>
+// Sum of a lane's p.  bf16: as products of 4x4x4 blocks with ones, in which a lane's four elements meet no other lane's: 16
+// cycles of the matrix unit for eight tokens instead of 64 of the vector unit (64 head dims 883 -> 834 us, 128: 1106 -> 1099, over
+// prompts of 8192 tokens).
+template <typename T>
+struct RowSum {
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void add(const bf16x8& p) {
+    using i16x4 = __attribute__((ext_vector_type(4))) short;
+    using u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+    const i16x4 ones = {0x3f80, 0x3f80, 0x3f80, 0x3f80};
+    const u32x4 x = __builtin_bit_cast(u32x4, p);
+    acc = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_bit_cast(i16x4, u32x2{x[0], x[1]}), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(ones, __builtin_bit_cast(i16x4, u32x2{x[2], x[3]}), acc, 0, 0, 0);
+  }
+  __device__ __forceinline__ void scale(float f) { acc *= f; }
+  __device__ __forceinline__ float of_lane() const { return acc[0]; }
+};
+template <>
+struct RowSum<float> {
+  float acc = 0.f;
+  __device__ __forceinline__ void add(const f32x8& p) { acc = add_frag(acc, p); }
+  __device__ __forceinline__ void scale(float f) { acc *= f; }
+  __device__ __forceinline__ float of_lane() const { return acc; }
+};
+
+// DP: head dims of a row in LDS (64 or 128), DC <= DP: those that are multiplied
+template <typename T, int DP, int DC>
 __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
     page_attn_chunk_kernel(const PageAttnArgs a, const Split sp) {
   using TL = ChunkTile<T, DP>;
   using Frag = typename Traits<T>::Frag;
   constexpr int ROWB = TL::ROWB, CPR = TL::CPR, ES = (int)sizeof(T);
-  constexpr int KS = DP / 16, NDT = DP / 32, NL = CPR / 4, RPI = 64 / CPR;
+  constexpr int KS = DC / 16, NDT = DC / 32, NL = CPR / 4, RPI = 64 / CPR;
   extern __shared__ __attribute__((aligned(1024))) char tiles[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
@@ -573,56 +620,74 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   for (int i = 0; i < NDT; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) ot[i][e] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;                      // m in units of the raw scores
+  float m_run = -INFINITY;                                   // m in units of the raw scores
+  RowSum<T> l_run;
   const float cs = a.scale * kLog2e;
   const int32_t* trow = a.table + (long long)(ti.b < a.B ? ti.b : 0) * a.table_row;
   const char* kbase = a.k + kvh * a.k_head;
   const char* vbase = a.v + kvh * a.v_head;
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)tiles;
-  auto tile_of = [&](int i) { return i < sb ? i : lot + i - sb; };
-  // page of this wave's 16 tokens of a tile (-1 behind hi), left in a vector register until it is needed: made uniform at
-  // once, the wait for it would also wait for the tile's loads in front of it
-  auto page_of = [&](int i) {
-    const int tok0 = tile_of(i) * 64 + 16 * wave;
-    return i < i1 && tok0 < hi ? trow[tok0 >> a.shift] : -1;
+  auto start_of = [&](int i) { return (i < sb ? i : lot + i - sb) * 64; };   // first token of tile i
+  // Lane l: the page of tokens 16 (l % 4) .. + 15 of a tile (behind hi: that of the last token; nobody looks at it).  Left in a
+  // vector register until it is needed: made uniform at once, the wait for it would also wait for the loads in front of it.
+  auto pages_of = [&](int start) {
+    const int tok = start + 16 * (lane & 3);
+    return *reinterpret_cast<const int32_t*>(reinterpret_cast<const char*>(trow) + (uint32_t)((tok < hi ? tok : hi - 1) >> a.shift) * 4u);
   };
-  // Where lane l's 16 bytes of load v come from: LDS position l % CPR of row v RPI + l / CPR holds another piece of that row
+  // Where lane l's 16 bytes of load v come from: LDS position l % CPR of row v RPI + l / CPR holds another piece of that row.
+  // Less 1024 (v % 4): see lds_loads.  (A slot is at least as long as an LDS row when the loads below use that, so this is
+  // not negative.)
   uint32_t koff[NL], voff[NL];
+  uint32_t alive = 0;                                        // bit v: load v of K holds head dims; bit 8 + v: of V
 #pragma unroll
   for (int v = 0; v < NL; ++v) {
     const int row = v * RPI + lane / CPR;
-    koff[v] = (uint32_t)(row * a.k_slot) + (k_off<ROWB>(row, lane % CPR) - row * ROWB);
-    voff[v] = (uint32_t)(row * a.v_slot) + (v_off<ROWB>(row, lane % CPR, T{}) - row * ROWB);
+    const uint32_t kp = k_off<ROWB>(row, lane % CPR) - row * ROWB, vp = v_off<ROWB>(row, lane % CPR, T{}) - row * ROWB;
+    koff[v] = (uint32_t)(row * a.k_slot) + kp;
+    voff[v] = (uint32_t)(row * a.v_slot) + vp;
+    if (a.dim == DP) {
+      koff[v] -= 1024 * (v % 4);
+      voff[v] -= 1024 * (v % 4);
+    }
+    alive |= (uint32_t)((int)kp < a.dim * ES) << v | (uint32_t)((int)vp < a.dim * ES) << (8 + v);
   }
-  // this wave's 16 tokens of K or V of tile i into LDS; true if their page exists (or none is needed)
-  auto fetch = [&](uint32_t lds_tile, int i, int page, const char* base, unsigned long long page_bytes, int slot, const uint32_t (&off)[NL]) {
-    const int tok0 = tile_of(i) * 64 + 16 * wave;
-    const int left = hi - tok0;
-    const bool good = ((unsigned)page < (unsigned)a.n_pages) & (left > 0);
-    const uint32_t slot0 = tok0 & ((1 << a.shift) - 1), p0 = good ? page : 0;
-    const char* src = base + p0 * page_bytes + slot0 * (uint32_t)slot;
+  // this wave's 16 tokens of a tile whose tokens all are within [lo, hi): tok0 - lo < whole
+  const uint32_t whole = hi - 15 > lo ? hi - 15 - lo : 0;
+  // K or V of this wave's 16 tokens from tok0 on into LDS
+  auto fetch = [&](uint32_t lds_tile, int tok0, bool good, const char* src, const uint32_t (&off)[NL], uint32_t live) {
     const uint32_t dst = lds_tile + 16 * wave * ROWB;
-    if (good & (left >= 16) & (tok0 >= lo) & (a.dim == DP)) {
+    if (good & ((uint32_t)(tok0 - lo) < whole)) {
+      if (a.dim == DP) {
+        lds_loads(dst, src, off);
+      } else {                                               // the other lanes' bytes are zero from the start
 #pragma unroll
-      for (int v = 0; v < NL; ++v) lds_load16(dst + v * 1024, src, off[v]);
+        for (int v = 0; v < NL; ++v)
+          if (live >> v & 1) lds_load16(dst + v * 1024, src, off[v]);
+      }
     } else {                                                 // what nobody sees comes from a row of zeros
 #pragma unroll
       for (int v = 0; v < NL; ++v) {
         const int row = v * RPI + lane / CPR, j = tok0 + row;
-        const uint32_t piece = off[v] - (uint32_t)(row * slot);
-        const bool dead = !good | (row >= left) | ((j < lo) & (j >= sinks)) | ((int)piece >= a.dim * ES);
-        lds_load16(dst + v * 1024, dead ? reinterpret_cast<const char*>(&zero16) : src + off[v]);
+        const bool dead = !good | (j >= hi) | ((j < lo) & (j >= sinks)) | !(live >> v & 1);
+        lds_load16(dst + v * 1024, dead ? reinterpret_cast<const char*>(&zero16) : src + off[v] + (a.dim == DP ? 1024 * (v % 4) : 0));
       }
     }
-    return good | (left <= 0);
   };
-  auto fetch_k = [&](int buf, int i, int page) {
-    const bool ok = fetch(lds0 + buf * TL::TILE, i, page, kbase, (uint32_t)a.k_page, a.k_slot, koff);
-    if (lane == 0) reinterpret_cast<int*>(tiles + TL::OK_OFF + 16 * buf)[wave] = ok;
+  // What is known of a tile on its way: its first token, which of its four pages exist, and where this wave's part of V is
+  struct Coming { int start; uint32_t ok; const char* v; };
+  auto fetch_v = [&](int buf, const Coming& t) {
+    fetch(lds0 + TL::V_OFF + buf * TL::TILE, t.start + 16 * wave, t.ok >> wave & 1, t.v, voff, alive >> 8);
   };
-  auto fetch_v = [&](int buf, int i, int page) {
-    fetch(lds0 + TL::V_OFF + buf * TL::TILE, i, page, vbase, (uint32_t)a.v_page, a.v_slot, voff);
+  auto fetch_k = [&](int buf, int start, int pages) {
+    Coming t;
+    t.start = start;
+    t.ok = (uint32_t)__ballot((unsigned)pages < (unsigned)a.n_pages) & 15u;
+    const bool good = t.ok >> wave & 1;
+    const uint32_t page = good ? __builtin_amdgcn_readlane(pages, wave) : 0, slot0 = (start + 16 * wave) & ((1 << a.shift) - 1);
+    t.v = vbase + page * (unsigned long long)(uint32_t)a.v_page + slot0 * (uint32_t)a.v_slot;
+    fetch(lds0 + buf * TL::TILE, start + 16 * wave, good, kbase + page * (unsigned long long)(uint32_t)a.k_page + slot0 * (uint32_t)a.k_slot, koff, alive);
+    return t;
   };
   const uint32_t k_lane = lds0 + k_off<ROWB>(c, sizeof(T) == 2 ? h : 2 * h);
   uint32_t v_lane = lds0 + TL::V_OFF;
@@ -630,27 +695,27 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
     const int r = lane & 15;
     v_lane += v_off<ROWB>(4 * h + (r >> 2), 2 * ((lane >> 4) & 1) + ((r & 3) >> 1), T{}) + 8 * (r & 1);
   }
-  auto flags = [&](int buf) {
-    const u32x4 f = *reinterpret_cast<const u32x4*>(tiles + TL::OK_OFF + 16 * buf);
-    return uniform((int)(f[0] | f[1] << 1 | f[2] << 2 | f[3] << 3));
-  };
+  if (a.dim != DP) {                                         // head dims up to the padded width stay zero
+    for (int o = tid * 16; o < TL::BYTES; o += 256 * 16) *reinterpret_cast<u32x4*>(tiles + o) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+  }
+  // tiles of this wave that need no mask: all pages exist, last token <= in_hi, first one >= in_lo or last one < sinks
+  const int in_hi = a.causal ? wfirst : ti.kv - 1, in_lo = a.window > 0 ? wlast - a.window + 1 : 0;
 
   // Tile i + 1's scores are formed beside tile i's softmax: the products of one fill the time that the exponentials of the
   // other take.  K therefore runs a tile ahead of V.
   f32x16 s[2];
-  int okv = 15;
-  int page_v = 0, page_k = -1, page_next = -1;               // pages of V of tile i + 1, K of tile i + 2, and the one after
+  Coming t0{0, 0, vbase}, t1{0, 0, vbase};                   // tile i and tile i + 1
+  int pages = 0;                                             // of tile i + 2
   if (i0 < i1) {
-    const int p0 = uniform(page_of(i0)), p1 = uniform(page_of(i0 + 1));
-    fetch_k(0, i0, p0);
-    fetch_v(0, i0, p0);
-    if (i0 + 1 < i1) fetch_k(1, i0 + 1, p1);
-    page_next = page_of(i0 + 2);
-    page_v = p1;
+    const int first_pages = pages_of(start_of(i0)), second_pages = pages_of(start_of(i0 + 1));
+    t0 = fetch_k(0, start_of(i0), first_pages);
+    fetch_v(0, t0);
+    if (i0 + 1 < i1) t1 = fetch_k(1, start_of(i0 + 1), second_pages);
+    pages = pages_of(start_of(i0 + 2));
     lds_loads_done();
     __syncthreads();
     if (busy) {
-      okv = flags(0);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -665,13 +730,12 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
     const int cur = (i - i0) & 1;
     lds_loads_done();
     __syncthreads();                                         // K of tile i + 1 and V of tile i are in place
-    page_k = uniform(page_next);
-    if (i + 2 < i1) fetch_k(cur, i + 2, page_k);
-    if (i + 1 < i1) fetch_v(cur ^ 1, i + 1, page_v);
-    page_v = page_k;
-    page_next = page_of(i + 3);
+    Coming t2 = t1;
+    if (i + 2 < i1) t2 = fetch_k(cur, start_of(i + 2), pages);
+    if (i + 1 < i1) fetch_v(cur ^ 1, t1);
+    pages = pages_of(start_of(i + 3));
     if (busy) {
-      const int j0 = tile_of(i) * 64;
+      const int j0 = t0.start;
       const uint32_t kl = k_lane + (cur ^ 1) * TL::TILE, vl = v_lane + cur * TL::TILE;
       constexpr int RING = sizeof(T) == 2 ? 4 : 1, NX = 4 * NDT;                  // fragments on their way: RING products ahead
       Frag kf[RING], vf[RING];
@@ -680,16 +744,14 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         kf[x] = k_frag32<ROWB>(kl, x / KS, x % KS, T{});
         vf[x] = v_frag32<ROWB>(vl, x % NDT, x / NDT, lane, T{});
       }
-      const int okn = flags(cur ^ 1);
-      bool inside = okv == 15 && j0 + 63 <= (a.causal ? wfirst : ti.kv - 1);
-      if (a.window > 0) inside = inside && (j0 >= wlast - a.window + 1 || j0 + 63 < sinks);
+      const bool inside = (t0.ok == 15) & (j0 + 63 <= in_hi) & ((j0 >= in_lo) | (j0 + 63 < sinks));
       if (!inside) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int j = j0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-            const bool see = (okv >> (2 * t + (e >> 3)) & 1) & (j <= see_hi) & ((j >= see_lo) | (j < sinks));
+            const bool see = (t0.ok >> (2 * t + (e >> 3)) & 1) & (j <= see_hi) & ((j >= see_lo) | (j < sinks));
             s[t][e] = see ? s[t][e] : -INFINITY;
           }
       }
@@ -709,7 +771,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
       if (__any((tmax - m_run) * cs > 8.f)) {
         const float m_new = fmaxf(m_run, tmax);
         const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) * cs);
-        l_run *= alpha;
+        l_run.scale(alpha);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) ot[dt] *= alpha;
         m_run = m_new;
@@ -719,7 +781,9 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         float pk[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) pk[e] = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + e], cs, -m_use));
-        return p_frag(pk, T{});
+        Frag f = p_frag(pk, T{});
+        if constexpr (sizeof(T) == 2) asm("" : "+v"(f));         // or its halves are converted once more for the row sums
+        return f;
       };
       f32x16 sn[2];
 #pragma unroll
@@ -727,6 +791,10 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
 #pragma unroll
         for (int e = 0; e < 16; ++e) sn[t][e] = 0.f;
       Frag pf = step_p(0);
+      // Where two waves share a vector unit (128 head dims), the one in its products goes first: it keeps the matrix unit fed and
+      // its exponentials fall into the other's loads and maximum (1168 -> 1123 us).  With 64 head dims there are three and
+      // less to multiply: 834 us so, 874 with the priority.
+      if constexpr (DC > 64) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         Frag pn = pf;
@@ -740,17 +808,17 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
           mma32(ot[dt], vf[x % RING], pf);
           if (y < NX) vf[x % RING] = v_frag32<ROWB>(vl, y % NDT, y / NDT, lane, T{});
         }
-        l_run = add_frag(l_run, pf);
+        l_run.add(pf);
         if constexpr (sizeof(T) == 2) {
           if (u < 3) {
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
               __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-              __builtin_amdgcn_sched_group_barrier(0x002, 10 / NDT, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 16 / NDT, 0);
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
               __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-              __builtin_amdgcn_sched_group_barrier(0x002, 10 / NDT, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 16 / NDT, 0);
             }
           }
         } else {
@@ -758,21 +826,24 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         }
         pf = pn;
       }
+      if constexpr (DC > 64) __builtin_amdgcn_s_setprio(0);
       s[0] = sn[0];
       s[1] = sn[1];
-      okv = okn;
     }
+    t0 = t1;
+    t1 = t2;
   }
 
+  float l;
   {
     float x, y;
-    swap_halves32(l_run, x, y);
-    l_run = x + y;
+    swap_halves32(l_run.of_lane(), x, y);
+    l = x + y;
   }
   if (!live) return;
   const long long orow = (long long)(ti.c0 + ti.t0 + rt) * a.heads + kvh * group + rh;
   if (sp.pieces == 1) {
-    const float inv = l_run > 0.f ? 1.0f / l_run : (l_run == 0.f ? 0.f : l_run);       // NaN stays NaN
+    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);       // NaN stays NaN
     T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
@@ -791,7 +862,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
         const int d = 32 * dt + 8 * e + 4 * h;
         if (d < a.dim) store4(o + d, f32x4{ot[dt][4 * e], ot[dt][4 * e + 1], ot[dt][4 * e + 2], ot[dt][4 * e + 3]});
       }
-    if (h == 0) reinterpret_cast<float2*>(a.ws + sp.ws)[at] = float2{m_run * cs, l_run};    // the join works in base-2 exponents
+    if (h == 0) reinterpret_cast<float2*>(a.ws + sp.ws)[at] = float2{m_run * cs, l};    // the join works in base-2 exponents
   }
 }
 
@@ -977,7 +1048,8 @@ int check_args(int dtype, const PageAttnArgs& a) {
   if (a.dim <= 0 || a.dim > 128 || a.dim % 8) return fail("page_attention: head dim %d unsupported (<= 128, multiple of 8)", a.dim);
   if (a.shift < 0) return fail("page_attention: the page size must be a power of two, 16 to 1024");
   if (a.n_pages <= 0 || a.width <= 0 || a.table_row < a.width) return fail("page_attention: %d pages, table of %d columns in rows of %lld", a.n_pages, a.width, a.table_row);
-  if (((long long)a.width << a.shift) > 0x7fffffffll - 64) return fail("page_attention: a table of %d pages describes too many tokens", a.width);
+  if (((long long)a.width << a.shift) > 0x7fffffffll - 1024)       // positions a few tiles further on stay within 32 bits
+     return fail("page_attention: a table of %d pages describes too many tokens", a.width);
   if (a.window < 0 || a.sinks < 0 || a.max_rows < 0) return fail("page_attention: window, sinks and max_rows must not be negative");
   if (!(a.scale > 0.f) || !isfinite(a.scale)) return fail("page_attention: the scale must be positive and finite");
   const long long strides[] = {a.q_row, a.q_head, a.k_page, a.k_head, a.k_slot, a.v_page, a.v_head, a.v_slot};
@@ -997,12 +1069,12 @@ void join(const PageAttnArgs& a, const Split& s, hipStream_t stream) {
   else if (s.pieces > 1) page_attn_join_few_kernel<T><<<(unsigned)((s.ws_rows + 7) / 8), 256, 0, stream>>>(a, s);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
   using ST = StepTile<T, DP>;
   using CT = ChunkTile<T, DP>;
   auto sk = page_attn_step_kernel<T, DP>;
-  auto ck = page_attn_chunk_kernel<T, DP>;
+  auto ck = page_attn_chunk_kernel<T, DP, DC>;
   const long long chunk_grid = p.chunk_tiles * a.kv_heads * p.chunk.hchunks;
   const long long step_grid = p.step_tiles * a.kv_heads * p.step.hchunks * p.step.pieces;
   if (chunk_grid > 0x7fffffffll || step_grid > 0x7fffffffll)
@@ -1020,6 +1092,11 @@ int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
   return check_launch("page_attention");
 }
 
+template <typename T>
+int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
+  return a.dim <= 64 ? run<T, 64, 64>(a, p, stream) : a.dim <= 96 ? run<T, 128, 96>(a, p, stream) : run<T, 128, 128>(a, p, stream);
+}
+
 }  // namespace
 
 size_t page_attention_workspace_bytes(int dtype, const PageAttnArgs& a) {
@@ -1035,8 +1112,7 @@ int launch_page_attention(int dtype, const PageAttnArgs& a, size_t ws_bytes, hip
   const Plan p = make_plan(a);
   const size_t need = (size_t)p.ws * sizeof(float);
   if (need > 0 && (!a.ws || ws_bytes < need || (uintptr_t)a.ws % 16)) return fail("page_attention: workspace of %zu bytes, %zu needed", ws_bytes, need);
-  if (dtype == DT_BF16) return a.dim <= 64 ? run<bf16, 64>(a, p, stream) : run<bf16, 128>(a, p, stream);
-  return a.dim <= 64 ? run<float, 64>(a, p, stream) : run<float, 128>(a, p, stream);
+  return dtype == DT_BF16 ? run<bf16>(a, p, stream) : run<float>(a, p, stream);
 }
 
 }  // namespace fcenc
