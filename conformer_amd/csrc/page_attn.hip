@@ -43,7 +43,8 @@ constexpr int CHUNK_MIN = 32;               // requests with more rows (times he
 // the chunk at most; 2: the longer ones and the rows behind the last request.
 struct Split {
   int gc = 1, hchunks = 1, tt = 1, share = 0, per_request = 0;
-  int pieces = 1;                            // of the key axis; > 1: partial results go to the workspace from float `ws` on
+  int pieces = 1;                            // of the key axis, at most; the results of more than one go to the workspace from float `ws` on
+  int piece = 1 << 30;                       // longest piece, in the kernel's blocks of tokens
   long long ws = 0;
   long long ws_rows = 0;                     // (row, head) pairs there: all of them, or per_request rows of every request
 };
@@ -54,6 +55,36 @@ __device__ __host__ __forceinline__ long long ws_sums(long long rows, int pieces
 struct TileInfo {
   int b, t0, n, c0, kv;                      // request (B: rows behind the last one), first row, rows, offset, tokens
 };
+
+constexpr int STEP_BLOCK = 5, CHUNK_BLOCK = 6;               // log2 of the tokens that the kernels take at a time
+
+// The tokens that some row of a tile sees, [0, sinks) and [lo, hi), as `count` blocks: the first `sb`, then those from `lob` on.
+struct Span {
+  int first, last, lo, hi, sinks, sb, lob, count;
+};
+__device__ __forceinline__ Span span_of(const PageAttnArgs& a, const TileInfo& ti, int tt, int log) {
+  Span s;
+  s.first = ti.kv - ti.n + ti.t0;                            // position of the tile's first row
+  s.last = s.first + (ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt) - 1;
+  s.hi = a.causal ? s.last + 1 : ti.kv;
+  if (ti.b == a.B || s.hi < 0) s.hi = 0;
+  s.lo = a.window > 0 && s.first > 0 ? s.first - a.window + 1 : 0;
+  s.lo = s.lo < 0 ? 0 : (s.lo > s.hi ? s.hi : s.lo);
+  s.sinks = a.window > 0 ? a.sinks : 0;
+  const int up = (1 << log) - 1;
+  s.lob = s.lo >> log;
+  s.sb = ((s.sinks < s.hi ? s.sinks : s.hi) + up) >> log;
+  s.sb = s.sb < s.lob ? s.sb : s.lob;
+  s.count = s.hi > 0 ? s.sb + ((s.hi + up) >> log) - s.lob : 0;
+  return s;
+}
+// Pieces of a tile's key axis: equal ones, none longer than sp.piece as far as sp.pieces are enough (so a long request does not hold up
+// the launch, and a short one needs no join).
+__device__ __forceinline__ int pieces_of(const Split& sp, int count) {
+  if (sp.pieces == 1) return 1;
+  const int n = (count + sp.piece - 1) / sp.piece;
+  return n < 1 ? 1 : (n > sp.pieces ? sp.pieces : n);
+}
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int clamp_rows(int v, int rows) { return v < 0 ? 0 : (v > rows ? rows : v); }
@@ -188,14 +219,12 @@ struct StepTile {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 ? 1 : 2))
-    page_attn_step_kernel(const PageAttnArgs a, const Split sp) {
+__device__ __forceinline__ void step_tile(const PageAttnArgs& a, const Split& sp, unsigned block, char* smem) {
   using TL = StepTile<T, DP>;
   using Frag = typename Traits<T>::Frag;
   constexpr int ROWB = TL::ROWB, CPR = TL::CPR, ES = (int)sizeof(T);
   constexpr int KS = DP / 32, NDB = DP / 16, NV = CPR / 4;   // k32 steps, 16-dim blocks, V loads per 16 tokens
   constexpr int RPI = 64 / CPR;                              // V rows per load instruction
-  extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int g = lane >> 4, r = lane & 15;
@@ -203,25 +232,18 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
   // pieces fastest, tiles slowest: workgroups go round the 8 XCDs by their number, and with the tile (of which some are
   // empty) in front, a batch of two requests left half of the XCDs without work (164 against 100 us at 2 x 131072 tokens)
   const unsigned per_tile = a.kv_heads * sp.hchunks * sp.pieces;
-  const int tile = (int)(blockIdx.x / per_tile);
-  const int rest = (int)(blockIdx.x - tile * per_tile), column = rest / sp.pieces, split = rest - column * sp.pieces;
+  const int tile = (int)(block / per_tile);
+  const int rest = (int)(block - tile * per_tile), column = rest / sp.pieces, split = rest - column * sp.pieces;
   const int kvh = column / sp.hchunks, hc = column - kvh * sp.hchunks;
   const int group = a.heads / a.kv_heads;
 
   TileInfo ti;
   if (!find_tile(a, tile, sp, ti)) return;
-  const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
-  const int last = first + (ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt) - 1;
-  int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
-  if (ti.b == a.B || hi < 0) hi = 0;
-  int lo = a.window > 0 && first > 0 ? first - a.window + 1 : 0;
-  lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
-  const int sinks = a.window > 0 ? a.sinks : 0;
-  const int lob = lo >> 5;
-  int sb = ((sinks < hi ? sinks : hi) + 31) >> 5;
-  sb = sb < lob ? sb : lob;
-  const int count = hi > 0 ? sb + ((hi + 31) >> 5) - lob : 0;
-  const int i0 = (int)((long long)count * split / sp.pieces), i1 = (int)((long long)count * (split + 1) / sp.pieces);
+  const Span at_tile = span_of(a, ti, tt, STEP_BLOCK);
+  const int first = at_tile.first, last = at_tile.last, lo = at_tile.lo, hi = at_tile.hi, sinks = at_tile.sinks;
+  const int sb = at_tile.sb, lob = at_tile.lob, count = at_tile.count, pieces = pieces_of(sp, count);
+  if (split >= pieces) return;
+  const int i0 = (int)((long long)count * split / pieces), i1 = (int)((long long)count * (split + 1) / pieces);
 
   // this lane's row of the tile
   const int rt = r / gc, rh = hc * gc + r - rt * gc;
@@ -388,7 +410,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
     for (int d = 0; d < DPT; ++d) acc[d] += src[d] * f;
   }
   const long long orow = (long long)(ti.c0 + ti.t0 + ort) * a.heads + kvh * group + orh;
-  if (sp.pieces == 1) {
+  if (pieces == 1) {
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);       // NaN stays NaN
     T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
 #pragma unroll
@@ -402,6 +424,13 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
       if (d0 + d < a.dim) o[d0 + d] = acc[d];
     if ((tid & 15) == 0) reinterpret_cast<float2*>(a.ws + sp.ws)[at] = float2{m, l};
   }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 ? 1 : 2))
+    page_attn_step_kernel(const PageAttnArgs a, const Split sp) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  step_tile<T, DP>(a, sp, blockIdx.x, lds);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -557,39 +586,32 @@ struct RowSum<float> {
 
 // DP: head dims of a row in LDS (64 or 128), DC <= DP: those that are multiplied
 template <typename T, int DP, int DC>
-__global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
-    page_attn_chunk_kernel(const PageAttnArgs a, const Split sp) {
+__device__ __forceinline__ void chunk_tile(const PageAttnArgs& a, const Split& sp, unsigned block, unsigned blocks, char* tiles) {
   using TL = ChunkTile<T, DP>;
   using Frag = typename Traits<T>::Frag;
   constexpr int ROWB = TL::ROWB, CPR = TL::CPR, ES = (int)sizeof(T);
   constexpr int KS = DC / 16, NDT = DC / 32, NL = CPR / 4, RPI = 64 / CPR;
-  extern __shared__ __attribute__((aligned(1024))) char tiles[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform(tid >> 6);
   const int h = lane >> 5, c = lane & 31;
   // workgroups of one kv head are dispatched to one XCD where the number of kv heads allows it (their tiles read the same
   // keys), long tiles (the late rows of a causal chunk) first
   const int columns = a.kv_heads * sp.hchunks;
-  const int tile = (int)((gridDim.x - 1 - blockIdx.x) / columns), column = (int)(blockIdx.x % columns);
+  const int split = (int)(block / blocks);
+  block -= split * blocks;
+  const int tile = (int)((blocks - 1 - block) / columns), column = (int)(block % columns);
   const int kvh = column / sp.hchunks, hc = column - kvh * sp.hchunks;
-  const int gc = sp.gc, tt = sp.tt, split = blockIdx.y;
+  const int gc = sp.gc, tt = sp.tt;
   const int group = a.heads / a.kv_heads;
 
   TileInfo ti;
   if (!find_tile(a, tile, sp, ti)) return;
-  const int first = ti.kv - ti.n + ti.t0;                    // position of the tile's first row
-  const int live_tt = ti.n - ti.t0 < tt ? ti.n - ti.t0 : tt;
-  const int last = first + live_tt - 1;
-  int hi = a.causal ? last + 1 : ti.kv;                      // tokens that some row sees: [0, sinks) and [lo, hi)
-  if (ti.b == a.B || hi < 0) hi = 0;
-  int lo = a.window > 0 && first > 0 ? first - a.window + 1 : 0;
-  lo = lo < 0 ? 0 : (lo > hi ? hi : lo);
-  const int sinks = a.window > 0 ? a.sinks : 0;
-  const int lot = lo >> 6;
-  int sb = ((sinks < hi ? sinks : hi) + 63) >> 6;
-  sb = sb < lot ? sb : lot;
-  const int count = hi > 0 ? sb + ((hi + 63) >> 6) - lot : 0;
-  const int i0 = (int)((long long)count * split / sp.pieces), i1 = (int)((long long)count * (split + 1) / sp.pieces);
+  const Span at_tile = span_of(a, ti, tt, CHUNK_BLOCK);
+  const int first = at_tile.first, lo = at_tile.lo, hi = at_tile.hi, sinks = at_tile.sinks;
+  const int sb = at_tile.sb, lot = at_tile.lob, count = at_tile.count, pieces = pieces_of(sp, count);
+  if (split >= pieces) return;
+  const int live_tt = at_tile.last - first + 1;
+  const int i0 = (int)((long long)count * split / pieces), i1 = (int)((long long)count * (split + 1) / pieces);
 
   // this lane's row and this wave's rows
   const int R = 32 * wave + c;
@@ -842,7 +864,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   }
   if (!live) return;
   const long long orow = (long long)(ti.c0 + ti.t0 + rt) * a.heads + kvh * group + rh;
-  if (sp.pieces == 1) {
+  if (pieces == 1) {
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);       // NaN stays NaN
     T* o = reinterpret_cast<T*>(a.out) + orow * a.dim;
 #pragma unroll
@@ -866,37 +888,71 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : 2))
   }
 }
 
-// The output row of a (row, head) pair of a launch's workspace; -1 if nothing was written there.
-__device__ __forceinline__ int joined_row(const PageAttnArgs& a, const Split& sp, int wrow) {
+// Workgroups of the short requests behind those of the long ones: they are bound by memory and fill what the last chunks
+// leave idle (12 requests, half of them single tokens, up to 512 rows and 16384 tokens: 558 us in two launches, 510 in one).
+template <typename T, int DP, int DC>
+__global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : ChunkTile<T, DP>::ROWB > 128 ? 2 : 3))
+    page_attn_chunk_kernel(const PageAttnArgs a, const Split sp, const Split step, const unsigned blocks) {
+  static_assert(ChunkTile<T, DP>::BYTES >= StepTile<T, DP>::BYTES, "one size of LDS for both");
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const unsigned chunks = blocks * sp.pieces;
+  if (__builtin_expect(blockIdx.x >= chunks, 0)) {
+    step_tile<T, DP>(a, step, blockIdx.x - chunks, lds);
+    return;
+  }
+  chunk_tile<T, DP, DC>(a, sp, blockIdx.x, blocks, lds);
+}
+
+// The output row of row `wrow` of a launch's workspace and how many pieces its results are in; 0: it is written already.
+__device__ __forceinline__ int joined_pieces(const PageAttnArgs& a, const Split& sp, int wrow, int log, int& row) {
+  TileInfo ti;
   if (sp.share == 1) {
-    const int b = wrow / sp.per_request, i = wrow - b * sp.per_request;
-    const int c0 = clamp_rows(a.cu_rows[b], a.rows), n = clamp_rows(a.cu_rows[b + 1], a.rows) - c0;
-    return i < n && n <= sp.per_request ? c0 + i : -1;
-  }
-  if (sp.share == 2) {
-    int lo = 0, hi = a.B + 1;                                // the request of this row (B: behind the last one)
+    ti.b = wrow / sp.per_request;
+    row = wrow - ti.b * sp.per_request;
+    ti.c0 = clamp_rows(a.cu_rows[ti.b], a.rows);
+    ti.n = clamp_rows(a.cu_rows[ti.b + 1], a.rows) - ti.c0;
+    if (row >= ti.n || ti.n > sp.per_request) return 0;
+    row += ti.c0;
+  } else {
+    // the last request that starts at or before this row (B: behind all of them), 32 candidates at a time
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = a.B + 1;
     while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.cu_rows[mid] <= wrow) lo = mid; else hi = mid;
+      const int step = (hi - lo + 31) >> 5, b = lo + lane * step;
+      const unsigned long long starts = __ballot(b < hi && a.cu_rows[b] <= wrow);
+      const int k = __popc((unsigned)(starts >> (threadIdx.x & 32))) - 1;
+      lo += (k > 0 ? k : 0) * step;
+      hi = hi < lo + step ? hi : lo + step;
     }
-    if (lo < a.B && clamp_rows(a.cu_rows[lo + 1], a.rows) - clamp_rows(a.cu_rows[lo], a.rows) <= sp.per_request) return -1;
+    row = wrow;
+    if (lo == a.B) return 0;
+    ti.b = lo;
+    ti.c0 = clamp_rows(a.cu_rows[lo], a.rows);
+    ti.n = clamp_rows(a.cu_rows[lo + 1], a.rows) - ti.c0;
+    if (row - ti.c0 >= ti.n || (sp.share == 2 && ti.n <= sp.per_request)) return 0;
   }
-  return wrow;
+  ti.t0 = (row - ti.c0) / sp.tt * sp.tt;
+  const int cap = a.width << a.shift, kv = a.kv_lens[ti.b];
+  ti.kv = kv < 0 ? 0 : (kv > cap ? cap : kv);
+  const int n = pieces_of(sp, span_of(a, ti, sp.tt, log).count);
+  return n > 1 ? n : 0;
 }
 
 // Joins few pieces: 32 threads per (row, head), four dims each.  (A workgroup per pair, as below, moved 1 TB/s of the
 // partial results of 80 000 pairs x 3 pieces.)
 constexpr int JOIN_FEW = 32;
 template <typename T>
-__global__ __launch_bounds__(256) void page_attn_join_few_kernel(const PageAttnArgs a, const Split sp) {
-  const long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, pieces = sp.pieces, d = lane * 4;
-  if (at >= sp.ws_rows) return;
+__global__ __launch_bounds__(256) void page_attn_join_few_kernel(const PageAttnArgs a, const Split sp, const int log) {
+  const long long slot = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const bool there = slot < sp.ws_rows;
+  const long long at = there ? slot : 0;                     // (all lanes of a wave take part in the search for the request)
+  const int lane = threadIdx.x & 31, d = lane * 4;
   const int wrow = (int)(at / a.heads), head = (int)(at - (long long)wrow * a.heads);
-  const int row = joined_row(a, sp, wrow);
-  if (row < 0) return;
+  int row;
+  const int pieces = joined_pieces(a, sp, wrow, log, row);
+  if (!there || pieces == 0) return;
   float2 p{-INFINITY, 0.f};
-  if (lane < pieces) p = reinterpret_cast<const float2*>(a.ws + sp.ws)[at * pieces + lane];
+  if (lane < pieces) p = reinterpret_cast<const float2*>(a.ws + sp.ws)[at * sp.pieces + lane];
   float m = p.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 32));
@@ -905,7 +961,7 @@ __global__ __launch_bounds__(256) void page_attn_join_few_kernel(const PageAttnA
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor(l, o, 32);
   const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-  const float* src = a.ws + sp.ws + ws_sums(sp.ws_rows, pieces) + at * pieces * a.dim + d;
+  const float* src = a.ws + sp.ws + ws_sums(sp.ws_rows, sp.pieces) + at * sp.pieces * a.dim + d;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int k0 = 0; k0 < pieces; k0 += 4) {
     f32x4 v[4];
@@ -926,16 +982,17 @@ __global__ __launch_bounds__(256) void page_attn_join_few_kernel(const PageAttnA
 // Joins many pieces: a workgroup per (row, head).  32 threads hold the dims, four each; the eight groups of 32 take every
 // eighth piece, four loads in flight, and meet in LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs a, const Split sp) {
+__global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs a, const Split sp, const int log) {
   __shared__ float s_m[4], s_l[4];
   __shared__ float s_w[MAX_SPLITS];
   __shared__ f32x4 s_acc[8][32];
-  const int at = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pieces = sp.pieces;
+  const int at = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wrow = at / a.heads, head = at - wrow * a.heads;
-  const int row = joined_row(a, sp, wrow);
-  if (row < 0) return;
+  int row;
+  const int pieces = joined_pieces(a, sp, wrow, log, row);
+  if (pieces == 0) return;
   float2 p{-INFINITY, 0.f};                                  // MAX_SPLITS pieces: one per thread
-  if (tid < pieces) p = reinterpret_cast<const float2*>(a.ws + sp.ws)[(long long)at * pieces + tid];
+  if (tid < pieces) p = reinterpret_cast<const float2*>(a.ws + sp.ws)[(long long)at * sp.pieces + tid];
   float m = p.x;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
@@ -954,7 +1011,7 @@ __global__ __launch_bounds__(256) void page_attn_join_kernel(const PageAttnArgs 
   const int g = tid >> 5, d = (tid & 31) * 4;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   if (d < a.dim) {
-    const float* src = a.ws + sp.ws + ws_sums(sp.ws_rows, pieces) + (long long)at * pieces * a.dim + d;
+    const float* src = a.ws + sp.ws + ws_sums(sp.ws_rows, sp.pieces) + (long long)at * sp.pieces * a.dim + d;
     for (int k0 = g; k0 < pieces; k0 += 32) {
       f32x4 v[4];
 #pragma unroll
@@ -985,20 +1042,24 @@ struct Plan {
 };
 
 // Pieces of the key axis for a launch with `busy` workgroups per piece, by the longest request that the table can
-// describe: enough to fill the chip with `fill` workgroups as long as a piece has 256 tokens, and up to 2048, which the
-// dispatcher can balance, as long as it has `least`.  Measured on single tokens (16 rows a tile, fill 512 = two per CU, least 2048):
-// 2 requests of up to 131072 tokens x 4 kv heads 77 us with 64 pieces, 90 with 256; 64 x 8192 x 8 262 us with 4, 272 with 2.
-int pieces_for(const PageAttnArgs& a, long long busy, int fill, int least) {
+// describe: enough to fill the chip with 512 workgroups (two per CU) as long as a piece has 256 tokens, and up to `most`, which
+// the dispatcher can balance, as long as it has 2048.  Single tokens: 2 requests of up to 131072 tokens x 4 kv heads 77 us with
+// 64 pieces, 90 with 256; 64 x 8192 x 8 262 us with 4, 272 with 2.  Chunks, in the example above: 520 us with 2560, 534 with 2048,
+// 542 with 4096, 567 with 6144.  Shorter requests have fewer pieces: chunks as many as keep each within the longest's, so that
+// no workgroup ends much later than the others; single tokens, which wait for memory only, down to 512 tokens each (64
+// requests of 1 to 8192 tokens 307 us, 318 with the longest's, both with caches cold).
+void divide(const PageAttnArgs& a, Split& s, long long busy, int most, int log) {
   long long longest = (long long)a.width << a.shift;
   const long long seen = (long long)a.window + a.sinks + CHUNK_ROWS;
   if (a.window > 0 && seen < longest) longest = seen;
   if (busy < 1) busy = 1;
-  long long n = fill / busy, m = 2048 / busy;
+  long long n = 512 / busy, m = most / busy;
   if (n > longest / 256) n = longest / 256;
-  if (m > longest / least) m = longest / least;
+  if (m > longest / 2048) m = longest / 2048;
   if (m > n) n = m;
   if (n > MAX_SPLITS) n = MAX_SPLITS;
-  return n < 1 ? 1 : (int)n;
+  s.pieces = n < 1 ? 1 : (int)n;
+  s.piece = (int)((((longest + (1 << log) - 1) >> log) + s.pieces - 1) / s.pieces);
 }
 
 long long ws_floats(const PageAttnArgs& a, const Split& s) {
@@ -1021,7 +1082,8 @@ Plan make_plan(const PageAttnArgs& a) {
     s.per_request = chunks ? few : 0;
     p.step_tiles = chunks ? (long long)a.B * ((few + s.tt - 1) / s.tt) : (long long)a.rows / s.tt + a.B + 1;
     const long long full = chunks ? 0 : (a.rows + s.tt - 1) / s.tt, some = a.rows < a.B ? a.rows : a.B;
-    s.pieces = pieces_for(a, (full > some ? full : some) * a.kv_heads * s.hchunks, 512, 2048);
+    divide(a, s, (full > some ? full : some) * a.kv_heads * s.hchunks, 2048, STEP_BLOCK);
+    s.piece = s.piece < 16 ? s.piece : 16;
     s.ws_rows = (chunks ? (long long)a.B * few : (long long)a.rows) * a.heads;
   }
   if (chunks) {
@@ -1032,7 +1094,7 @@ Plan make_plan(const PageAttnArgs& a) {
     s.share = 2;
     s.per_request = few;
     p.chunk_tiles = (long long)a.rows / s.tt + a.B + 1;
-    s.pieces = pieces_for(a, (long long)(a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 512, 2048);
+    divide(a, s, (long long)(a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 2560, CHUNK_BLOCK);
     s.ws_rows = (long long)a.rows * a.heads;
     s.ws = (ws_floats(a, p.step) + 3) & ~3ll;
   }
@@ -1064,9 +1126,9 @@ int check_args(int dtype, const PageAttnArgs& a) {
 }
 
 template <typename T>
-void join(const PageAttnArgs& a, const Split& s, hipStream_t stream) {
-  if (s.pieces > JOIN_FEW) page_attn_join_kernel<T><<<(unsigned)s.ws_rows, 256, 0, stream>>>(a, s);
-  else if (s.pieces > 1) page_attn_join_few_kernel<T><<<(unsigned)((s.ws_rows + 7) / 8), 256, 0, stream>>>(a, s);
+void join(const PageAttnArgs& a, const Split& s, int log, hipStream_t stream) {
+  if (s.pieces > JOIN_FEW) page_attn_join_kernel<T><<<(unsigned)s.ws_rows, 256, 0, stream>>>(a, s, log);
+  else if (s.pieces > 1) page_attn_join_few_kernel<T><<<(unsigned)((s.ws_rows + 7) / 8), 256, 0, stream>>>(a, s, log);
 }
 
 template <typename T, int DP, int DC>
@@ -1075,20 +1137,18 @@ int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
   using CT = ChunkTile<T, DP>;
   auto sk = page_attn_step_kernel<T, DP>;
   auto ck = page_attn_chunk_kernel<T, DP, DC>;
-  const long long chunk_grid = p.chunk_tiles * a.kv_heads * p.chunk.hchunks;
+  const long long chunk_blocks = p.chunk_tiles * a.kv_heads * p.chunk.hchunks;
   const long long step_grid = p.step_tiles * a.kv_heads * p.step.hchunks * p.step.pieces;
-  if (chunk_grid > 0x7fffffffll || step_grid > 0x7fffffffll)
-    return fail("page_attention: too many rows or heads");
+  if (chunk_blocks * p.chunk.pieces + step_grid > 0x7fffffffll) return fail("page_attention: too many rows or heads");
   if (p.chunk_tiles > 0) {
     if (reserve_lds(reinterpret_cast<const void*>(ck), CT::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", CT::BYTES);
-    ck<<<dim3((unsigned)chunk_grid, p.chunk.pieces), 256, CT::BYTES, stream>>>(a, p.chunk);
-    join<T>(a, p.chunk, stream);
-  }
-  if (p.step_tiles > 0) {
+    ck<<<(unsigned)(chunk_blocks * p.chunk.pieces + step_grid), 256, CT::BYTES, stream>>>(a, p.chunk, p.step, (unsigned)chunk_blocks);
+    join<T>(a, p.chunk, CHUNK_BLOCK, stream);
+  } else {
     if (reserve_lds(reinterpret_cast<const void*>(sk), ST::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", ST::BYTES);
     sk<<<(unsigned)step_grid, 64 * STEP_WAVES, ST::BYTES, stream>>>(a, p.step);
-    join<T>(a, p.step, stream);
   }
+  if (p.step_tiles > 0) join<T>(a, p.step, STEP_BLOCK, stream);
   return check_launch("page_attention");
 }
 
