@@ -678,6 +678,21 @@ __device__ __forceinline__ float value_at(int i) {
   return __builtin_bit_cast(float, u << 16);
 }
 
+// Two values at once, in packed 16-bit integers: the vector unit is busy for half of the time, waits fill the rest (with the
+// weights found by neighbouring lanes, 50 -> 46 us for 256 rows of 131072).
+using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
+using i16x2 = __attribute__((ext_vector_type(2))) short;
+__device__ __forceinline__ i16x2 both(int x) { return i16x2{(short)x, (short)x}; }
+__device__ __forceinline__ u16x2 magnitudes(unsigned u) { return __builtin_bit_cast(u16x2, u & 0x7fff7fffu); }
+// index_of of both
+__device__ __forceinline__ i16x2 indices_of(unsigned u) {
+  const u16x2 d = __builtin_elementwise_sub_sat(magnitudes(u), __builtin_bit_cast(u16x2, both(BV_LO - 1)));
+  unsigned negative = __builtin_bit_cast(unsigned, __builtin_bit_cast(i16x2, u) >> 15);    // all ones or none
+  asm("" : "+v"(negative));                                  // or it becomes two selects
+  // BV_ZERO + d or BV_ZERO - d = BV_ZERO + ~d + 1
+  return __builtin_bit_cast(i16x2, ~(__builtin_bit_cast(unsigned, d) ^ negative)) + __builtin_bit_cast(i16x2, negative) + both(BV_ZERO + 1);
+}
+
 // prefix sums over the bins of this thread's first one; lds.mass[0] becomes the whole mass
 __device__ __forceinline__ void before_mine(const ByValueLds& lds, unsigned c, u64 m, int wave, int lane, unsigned& cb, u64& mb) {
   const unsigned ci = wave_running(c, lane);
@@ -718,19 +733,19 @@ __device__ __forceinline__ bool sample_by_value(char* smem, const RowSource<bf16
   __syncthreads();
   // ---- one pass: count every value ----
   {
-    int least = 0;
-    bool odd = false;
+    i16x2 least = both(0);
+    u16x2 tiny = {0xffff, 0xffff};
     s.vectors(0, n, [&](int e, const u32x4& raw) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const unsigned v = bits16(raw, k);
-        const int i = index_of(v);
-        least = min(least, i);
-        odd |= (v & 0x7fffu) - 1u < (unsigned)BV_LO - 1u;                 // between 0 and 2^-30
-        atomicAdd(&lds.count[min(max(i, 0), BV_LOW)], 1u);                // -inf and NaN among the low ones, and what fills up the row
+      for (int k = 0; k < 4; ++k) {
+        const i16x2 i = indices_of(raw[k]), c = __builtin_elementwise_min(__builtin_elementwise_max(i, both(0)), both(BV_LOW));
+        least = __builtin_elementwise_min(least, i);
+        tiny = __builtin_elementwise_min(tiny, magnitudes(raw[k]) - u16x2{1, 1});       // of 0: 0xffff
+        atomicAdd(&lds.count[c.x], 1u);                      // -inf and NaN among the low ones, and what fills up the row
+        atomicAdd(&lds.count[c.y], 1u);
       }
     });
-    if (least < 0 || odd) lds.word[1] = 1;
+    if (least.x < 0 || least.y < 0 || tiny.x < BV_LO - 1 || tiny.y < BV_LO - 1) lds.word[1] = 1;      // 2^7 and more; between 0 and 2^-30
   }
   __syncthreads();
   unsigned cnt[BV_PER];
@@ -755,11 +770,13 @@ __device__ __forceinline__ bool sample_by_value(char* smem, const RowSource<bf16
 
   // ---- weights, and the borders ----
   unsigned c = 0;
+  // (values that occur lie close together: neighbours go to neighbouring lanes here)
+  for (int i = tid; i < BV_LOW; i += 64 * MAX_WAVES) lds.weight[i] = lds.count[i] ? rounded(weight_by(value_at(i), p, unit)) : 0;
+  __syncthreads();
   u64 m = 0, w[BV_PER];
 #pragma unroll
   for (int j = 0; j < BV_PER; ++j) {
-    const int i = tid * BV_PER + j;
-    w[j] = cnt[j] ? rounded(weight_by(value_at(i), p, unit)) : 0;
+    w[j] = cnt[j] ? lds.weight[tid * BV_PER + j] : 0;
     c += cnt[j];
     m += cnt[j] * w[j];
   }
@@ -863,17 +880,24 @@ __device__ __forceinline__ bool sample_by_value(char* smem, const RowSource<bf16
     target = target < total ? target : total - 1;
   }
   int from = 0, to = n;
+  const i16x2 last_kept = both(border);
   for (int level = 0; level < 2; ++level) {
     u64 sum = 0;
-    unsigned eq = 0;
+    unsigned seen = 0;
+    u16x2 others = {0, 0};
     s.vectors(from, to, [&](int e, const u32x4& raw) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int i = min(index_of(bits16(raw, k)), BV_LOW);
-        sum += lds.weight[i];
-        eq += i == border;
+      for (int k = 0; k < 4; ++k) {
+        const i16x2 i = indices_of(raw[k]);
+        const u16x2 c = __builtin_bit_cast(u16x2, __builtin_elementwise_min(i, last_kept));
+        unsigned apart = __builtin_bit_cast(unsigned, i ^ last_kept);
+        asm("" : "+v"(apart));                               // or the line after the next becomes comparisons
+        sum += lds.weight[c.x] + lds.weight[c.y];            // 0 from the border on; one address, so those lanes do not collide
+        others += __builtin_elementwise_min(__builtin_bit_cast(u16x2, apart), u16x2{1, 1});
       }
+      seen += 8;
     });
+    unsigned eq = seen - others.x - others.y;                // of the border's value
     sum = wave_total(sum);
     eq = wave_total(eq);
     __syncthreads();
