@@ -9,7 +9,8 @@
 //
 // One pass over the keys with a running maximum m and sum l per row (fp32, base-2 exponents):
 //     m' = max(m, max_j s_j),  l' = l 2^(m - m') + sum_j 2^(s_j - m'),  O' = O 2^(m - m') + sum_j 2^(s_j - m') v_j.
-// In bf16 the p_j = 2^(s_j - m') are rounded for the product with v, and l adds up the rounded ones: what is rounded off in the numerator is then missing in the denominator too, and a row that one key dominates loses nothing.
+// In bf16 the p_j = 2^(s_j - m') are rounded for the product with v, and l adds up the rounded ones: what is rounded off in
+// the numerator is then missing in the denominator too, and a row that one key dominates loses nothing.
 //
 // A tile is a set of rows of one (request, kv head): `tt` neighbouring rows of the chunk times the gc query heads that
 // share the kv head, so that a key read once serves all of them.  Workgroup t finds its request without any table:
@@ -20,9 +21,10 @@
 // rows, and those rows are, as they are, the k elements of the B operand of O^T = V^T P^T once the V fragment is read
 // in the same token order.  P never leaves the registers; V^T fragments come out of LDS with transposing reads.
 //
-// Loads of K and V go through a buffer descriptor per 16 tokens of a page (pages hold at least 16) whose size ends behind the
-// last token that the tile sees: what lies beyond (stale slots, head dims up to the padded width, bad pages) loads
-// as zero, so garbage there can reach neither the scores nor, as 0 * NaN, the sums.
+// K and V are looked up by 16 tokens (a page holds at least as many).  Of those, what no row of the tile sees (stale slots,
+// tokens in front of the window, bad pages, head dims up to the padded width) arrives as zero, so garbage there can reach
+// neither the scores nor, as 0 * NaN, the sums: in the step kernel by buffer descriptors that end behind the last token seen,
+// in the chunk kernel, which loads straight into LDS, by lanes that read a row of zeros instead.
 #include <math.h>
 
 #include "common.h"
@@ -207,7 +209,8 @@ __device__ __forceinline__ void store_row(float* p, float v) { *p = v; }
 // Tiles of up to 16 rows: single tokens and short chunks.  Bound by the bytes of K and V.  The four waves of a workgroup
 // take every fourth block of 32 tokens, on their own (K straight into MFMA fragments, V through a wave-private LDS
 // tile), with the next block's loads in flight; their partial results meet in LDS.  With few tiles the key axis is
-// also cut into `splits` pieces, whose results a second launch joins.
+// also cut into `splits` pieces, whose results a second launch joins.  64 requests of up to 8192 tokens, 8 kv heads of 128 in
+// bf16 under 32 heads: 257 us, 5.4 TB/s of K and V (a large copy reaches 5.2); 2 of up to 131072 over 4 kv heads: 75 us.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int DP>
 struct StepTile {
@@ -230,7 +233,7 @@ __device__ __forceinline__ void step_tile(const PageAttnArgs& a, const Split& sp
   const int g = lane >> 4, r = lane & 15;
   const int gc = sp.gc, tt = sp.tt;
   // pieces fastest, tiles slowest: workgroups go round the 8 XCDs by their number, and with the tile (of which some are
-  // empty) in front, a batch of two requests left half of the XCDs without work (164 against 100 us at 2 x 131072 tokens)
+  // empty) in front, a batch of two requests left half of the XCDs without work (146 against 77 us at 2 x 131072 tokens)
   const unsigned per_tile = a.kv_heads * sp.hchunks * sp.pieces;
   const int tile = (int)(block / per_tile);
   const int rest = (int)(block - tile * per_tile), column = rest / sp.pieces, split = rest - column * sp.pieces;
@@ -436,8 +439,11 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
 // ---------------------------------------------------------------------------------------------------------------
 // Tiles of up to 128 rows: chunks and prompts.  Four waves of 32 rows share each K / V tile of 64 tokens through LDS;
 // 32x32 MFMAs, so a wave reads a fragment once for 32 rows and a row's statistics need one exchange between the two
-// halves of the wave.  A tile is loaded into registers (wave w: tokens 16w .. 16w + 15, one page lookup) while the one
-// before it is multiplied, then written to LDS.
+// halves of the wave.  Tiles go from memory straight into LDS (wave w: tokens 16 w .. 16 w + 15, one page lookup), two of each
+// in flight or in use, K a tile ahead of V: the products for tile i + 1's scores stand beside tile i's exponentials.
+// Bound by the matrix and vector units together: at 128 head dims each is busy for about half of the time, and what one wave
+// needs of one the other wave of the SIMD must leave.  3 prompts of up to 8192 rows, 32 heads of 128 over 8, window 4096:
+// 0.88 ms, 1005 TFLOP/s in bf16, where a large matrix product reaches 1320; 85 in fp32 (143).
 //
 // C layout of a 32x32 product: lane (h = lane / 32, c = lane % 32), register i: row 8 (i / 4) + 4 h + i % 4, column c.  With
 // rows = tokens, registers 8 s .. 8 s + 7 are the eight tokens {4 h + 0..3, 8 + 4 h + 0..3} of 16-token step s: the k
@@ -942,8 +948,11 @@ __device__ __forceinline__ int joined_pieces(const PageAttnArgs& a, const Split&
 // partial results of 80 000 pairs x 3 pieces.)
 constexpr int JOIN_FEW = 32;
 template <typename T>
-__global__ __launch_bounds__(256) void page_attn_join_few_kernel(const PageAttnArgs a, const Split sp, const int log) {
-  const long long slot = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+__global__ __launch_bounds__(256) void page_attn_join_few_kernel(const PageAttnArgs a, const Split chunk, const Split step, const unsigned chunks) {
+  const bool of_chunk = blockIdx.x < chunks;
+  const Split& sp = of_chunk ? chunk : step;
+  const int log = of_chunk ? CHUNK_BLOCK : STEP_BLOCK;
+  const long long slot = (long long)(of_chunk ? blockIdx.x : blockIdx.x - chunks) * 8 + (threadIdx.x >> 5);
   const bool there = slot < sp.ws_rows;
   const long long at = there ? slot : 0;                     // (all lanes of a wave take part in the search for the request)
   const int lane = threadIdx.x & 31, d = lane * 4;
@@ -1125,10 +1134,15 @@ int check_args(int dtype, const PageAttnArgs& a) {
   return 0;
 }
 
+// few pieces of both launches' shares in one, many of either in one each
 template <typename T>
-void join(const PageAttnArgs& a, const Split& s, int log, hipStream_t stream) {
-  if (s.pieces > JOIN_FEW) page_attn_join_kernel<T><<<(unsigned)s.ws_rows, 256, 0, stream>>>(a, s, log);
-  else if (s.pieces > 1) page_attn_join_few_kernel<T><<<(unsigned)((s.ws_rows + 7) / 8), 256, 0, stream>>>(a, s, log);
+void join(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
+  const bool chunk = p.chunk_tiles > 0 && p.chunk.pieces > 1, step = p.step_tiles > 0 && p.step.pieces > 1;
+  if (chunk && p.chunk.pieces > JOIN_FEW) page_attn_join_kernel<T><<<(unsigned)p.chunk.ws_rows, 256, 0, stream>>>(a, p.chunk, CHUNK_BLOCK);
+  if (step && p.step.pieces > JOIN_FEW) page_attn_join_kernel<T><<<(unsigned)p.step.ws_rows, 256, 0, stream>>>(a, p.step, STEP_BLOCK);
+  const unsigned chunks = chunk && p.chunk.pieces <= JOIN_FEW ? (unsigned)((p.chunk.ws_rows + 7) / 8) : 0;
+  const unsigned steps = step && p.step.pieces <= JOIN_FEW ? (unsigned)((p.step.ws_rows + 7) / 8) : 0;
+  if (chunks + steps > 0) page_attn_join_few_kernel<T><<<chunks + steps, 256, 0, stream>>>(a, p.chunk, p.step, chunks);
 }
 
 template <typename T, int DP, int DC>
@@ -1143,12 +1157,11 @@ int run(const PageAttnArgs& a, const Plan& p, hipStream_t stream) {
   if (p.chunk_tiles > 0) {
     if (reserve_lds(reinterpret_cast<const void*>(ck), CT::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", CT::BYTES);
     ck<<<(unsigned)(chunk_blocks * p.chunk.pieces + step_grid), 256, CT::BYTES, stream>>>(a, p.chunk, p.step, (unsigned)chunk_blocks);
-    join<T>(a, p.chunk, CHUNK_BLOCK, stream);
   } else {
     if (reserve_lds(reinterpret_cast<const void*>(sk), ST::BYTES) != hipSuccess) return fail("page_attention: cannot reserve %d bytes of LDS", ST::BYTES);
     sk<<<(unsigned)step_grid, 64 * STEP_WAVES, ST::BYTES, stream>>>(a, p.step);
   }
-  if (p.step_tiles > 0) join<T>(a, p.step, STEP_BLOCK, stream);
+  join<T>(a, p, stream);
   return check_launch("page_attention");
 }
 
