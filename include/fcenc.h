@@ -474,13 +474,14 @@ int fcenc_mel_spectrogram(const fcenc_mel_plan* plan, const float* wave, long lo
  * fcenc_page_attention: request b has rows cu_rows[b] .. cu_rows[b + 1] - 1 of q (n of them) at positions
  * kv_lens[b] - n + i, its tokens (those rows' own K and V among them) already in the pages.  A row at position p sees
  * token j < kv_lens[b] if (not causal or j <= p) and (window == 0 or j > p - window or j < sinks); tokens of pages
- * whose id is outside the pool are seen by nobody.  out [rows][heads][head_dim] (dense); rows that see nothing and rows that
- * belong to no request are zeros.  What lies in slots that no row of the chunk sees is never used, whatever it is.  Among
- * the tokens that some row of the chunk sees, a key that is NaN or infinite reaches the rows that see it; a value (V) that
- * is may also reach rows of the same request and chunk that do not.  Query head h reads kv head h / (heads / kv_heads).  head_dim <= 128 and a
- * multiple of 8; all strides in elements, multiples of 16 bytes; scale > 0.  max_rows: the longest chunk of the batch if
- * the caller knows it, else 0 -- it chooses kernels and never changes what is computed.  The workspace (size from
- * fcenc_page_attention_workspace_bytes, may be 0) belongs to one call at a time.
+ * whose id is outside the pool are seen by nobody.  Query head h reads kv head h / (heads / kv_heads).
+ * out [rows][heads][head_dim] (dense); rows that see nothing and rows that belong to no request are zeros.  cu_rows starts at
+ * 0 and does not fall.  What lies in slots that no row of the chunk sees is never used, whatever it is.  Among the tokens
+ * that some row of the chunk sees, a key that is NaN or infinite reaches the rows that see it; a value (V) that is may also
+ * reach rows of the same request and chunk that do not.  head_dim <= 128 and a multiple of 8; all strides in elements,
+ * multiples of 16 bytes, of a page below 2^32 bytes; page_size slots of a head span at most 2 GiB; scale > 0.  max_rows: the
+ * longest chunk of the batch if the caller knows it, else 0 -- it chooses kernels and never changes what is computed.  The
+ * workspace (size from fcenc_page_attention_workspace_bytes, may be 0) belongs to one call at a time.
  *
  * fcenc_sample_tokens: one token per row of logits [rows][row_stride] (vocab <= 2^18 used).  With weights
  * w_i = exp((x_i - max) / temperature) and the order of falling logits (equal ones by rising index): top_k keeps the
