@@ -110,6 +110,30 @@ def test_attention_hint_changes_nothing_but_speed(max_rows):
     _check(got, q, kp, vp, table, kv, cu, 0.2, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [8, 32, 56, 72, 80, 96, 104, 128])
+@pytest.mark.parametrize("mask", [dict(), dict(window=100, sinks=70), dict(causal=False)])
+def test_attention_chunks_of_every_width(dtype, d, mask):
+    """Whole tiles of 64 tokens between ragged ones, at head dims that fill a row of the padded width and that do not."""
+    new, kv = [70, 33], [300, 257]
+    q, kp, vp, table, cu = _problem(dtype, 4, 2, d, 64, new, kv, 23)
+    _check(_run(q, kp, vp, table, kv, cu, d ** -0.5, **mask), q, kp, vp, table, kv, cu, d ** -0.5, dtype, **mask)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("extra_width", [40, 300])          # 24 pieces of the key axis at most, and 50
+@pytest.mark.parametrize("mask", [dict(), dict(window=3000, sinks=33)])
+def test_attention_pieces_by_length(dtype, extra_width, mask):
+    """Chunks and single tokens, long requests whose key axis is cut and short ones whose is not, empty ones and rows of nobody, in
+    one call."""
+    new, kv = [40, 1, 0, 3, 60, 2, 33, 1], [5000, 4000, 900, 20, 60, 3000, 700, 1]
+    q, kp, vp, table, cu = _problem(dtype, 8, 1, 64, 32, new, kv, 29, tail=3, extra_width=extra_width)
+    got = _run(q, kp, vp, table, kv, cu, 0.125, **mask)
+    assert (got[cu[-1]:] == 0).all()
+    _check(got[:cu[-1]], q[:cu[-1]], kp, vp, table, kv, cu, 0.125, dtype, **mask)
+    assert torch.equal(got, _run(q, kp, vp, table, kv, cu, 0.125, **mask))
+
+
 def test_attention_extreme_windows_and_unit_dimensions():
     """A window of 2^31 - 1 tokens is none, also where rows in front of the request's start share a tile with others; strides of
     dimensions of one element are not looked at."""
