@@ -94,35 +94,45 @@ __device__ __forceinline__ int clamp_rows(int v, int rows) { return v < 0 ? 0 : 
 // false: no such tile, or not of this launch's share
 __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const Split& sp, TileInfo& ti) {
   const int tt = sp.tt;
-  int lo = 0, hi = a.B + 1;
+  int lo = 0, c0, c1, kv;
   if (sp.share == 1) {                         // as many tiles for every request
     const int each = (sp.per_request + tt - 1) / tt;
     lo = tile / each;
-    tile = tile - lo * each + clamp_rows(uniform(a.cu_rows[lo]), a.rows) / tt + lo;
+    c0 = clamp_rows(uniform(a.cu_rows[lo]), a.rows);
+    c1 = clamp_rows(uniform(a.cu_rows[lo + 1]), a.rows);
+    kv = uniform(a.kv_lens[lo]);
+    tile = tile - lo * each + c0 / tt + lo;
   } else {
-    // 64 candidates at a time: one memory latency for up to 64 requests, two for up to 4096
+    // 64 candidates at a time, their lengths along with the last ones: one memory latency for up to 63 requests, two for up to
+    // 4095
     const int lane = threadIdx.x & 63;
+    int hi = a.B + 1, k = 0, start = 0, length = 0;
     while (hi - lo > 1) {
       const int step = (hi - lo + 63) >> 6;
       const int b = lo + lane * step;
-      const bool at_or_before = b < hi && clamp_rows(a.cu_rows[b], a.rows) / tt + b <= tile;
-      const int k = __popcll(__ballot(at_or_before)) - 1;     // starts rise with b
-      lo = lo + (k > 0 ? k : 0) * step;
+      if (b <= a.B) start = clamp_rows(a.cu_rows[b], a.rows);
+      if (step == 1 && b < a.B) length = a.kv_lens[b];
+      k = __popcll(__ballot(b < hi && start / tt + b <= tile)) - 1;     // starts rise with b
+      k = k > 0 ? k : 0;
+      lo = lo + k * step;
       hi = hi < lo + step ? hi : lo + step;
     }
+    k = uniform(k);
     lo = uniform(lo);
+    c0 = __builtin_amdgcn_readlane(start, k);
+    kv = __builtin_amdgcn_readlane(length, k);
+    c1 = lo == a.B ? a.rows : k < 63 ? __builtin_amdgcn_readlane(start, k + 1) : clamp_rows(uniform(a.cu_rows[lo + 1]), a.rows);
   }
   ti.b = lo;
-  ti.c0 = clamp_rows(uniform(a.cu_rows[lo]), a.rows);
-  const int c1 = lo < a.B ? clamp_rows(uniform(a.cu_rows[lo + 1]), a.rows) : a.rows;
-  ti.n = c1 - ti.c0;
-  ti.t0 = (tile - (ti.c0 / tt + lo)) * tt;
+  ti.c0 = c0;
+  ti.n = c1 - c0;
+  ti.t0 = (tile - (c0 / tt + lo)) * tt;
   ti.kv = 0;
   if (ti.t0 < 0 || ti.t0 >= ti.n) return false;
   if (sp.share == 1 && ti.n > sp.per_request) return false;
   if (sp.share == 2 && lo < a.B && ti.n <= sp.per_request) return false;
   if (lo < a.B) {
-    const int cap = a.width << a.shift, kv = uniform(a.kv_lens[lo]);
+    const int cap = a.width << a.shift;
     ti.kv = kv < 0 ? 0 : (kv > cap ? cap : kv);
   }
   return true;
