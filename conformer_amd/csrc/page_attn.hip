@@ -1064,9 +1064,10 @@ struct Plan {
 // describe: enough to fill the chip with 512 workgroups (two per CU) as long as a piece has 256 tokens, and up to `most`, which
 // the dispatcher can balance, as long as it has 2048.  Single tokens: 2 requests of up to 131072 tokens x 4 kv heads 77 us with
 // 64 pieces, 90 with 256; 64 x 8192 x 8 262 us with 4, 272 with 2.  Chunks, in the example above: 520 us with 2560, 534 with 2048,
-// 542 with 4096, 567 with 6144.  Shorter requests have fewer pieces: chunks as many as keep each within the longest's, so that
-// no workgroup ends much later than the others; single tokens, which wait for memory only, down to 512 tokens each (64
-// requests of 1 to 8192 tokens 307 us, 318 with the longest's, both with caches cold).
+// 542 with 4096, 567 with 6144.  Below 768 tokens the join costs more than it saves (one token, 32 heads of 64 over 8 kv
+// heads: 512 tokens 9.6 us cut, 7.8 whole; 1024 tokens 9.7 and 11.3).  Shorter requests have fewer pieces: chunks as many as
+// keep each within the longest's, so that no workgroup ends much later than the others; single tokens, which wait for memory
+// only, down to 512 tokens each (64 requests of 1 to 8192 tokens 307 us, 318 with the longest's, both with caches cold).
 void divide(const PageAttnArgs& a, Split& s, long long busy, int most, int log) {
   long long longest = (long long)a.width << a.shift;
   const long long seen = (long long)a.window + a.sinks + CHUNK_ROWS;
@@ -1077,6 +1078,7 @@ void divide(const PageAttnArgs& a, Split& s, long long busy, int most, int log) 
   if (m > longest / 2048) m = longest / 2048;
   if (m > n) n = m;
   if (n > MAX_SPLITS) n = MAX_SPLITS;
+  if (longest < 768) n = 1;
   s.pieces = n < 1 ? 1 : (int)n;
   s.piece = (int)((((longest + (1 << log) - 1) >> log) + s.pieces - 1) / s.pieces);
 }
