@@ -559,16 +559,16 @@ __device__ __forceinline__ void lds_loads(uint32_t dst, const char* base, const 
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 1\n\t"
         "global_load_lds_dwordx4 %1, %3\n\t"
-        "global_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(dst), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
+        "global_load_lds_dwordx4 %2, %3 offset:0x400" ::"s"(dst), "v"(off[0]), "v"(off[1]), "s"(base) : "memory");
   } else {
 #pragma unroll
     for (int v = 0; v < N; v += 4)
       asm volatile(
           "s_mov_b32 m0, %0\n\ts_nop 1\n\t"
           "global_load_lds_dwordx4 %1, %5\n\t"
-          "global_load_lds_dwordx4 %2, %5 offset:1024\n\t"
-          "global_load_lds_dwordx4 %3, %5 offset:2048\n\t"
-          "global_load_lds_dwordx4 %4, %5 offset:3072"
+          "global_load_lds_dwordx4 %2, %5 offset:0x400\n\t"
+          "global_load_lds_dwordx4 %3, %5 offset:0x800\n\t"
+          "global_load_lds_dwordx4 %4, %5 offset:0xc00"
           ::"s"(dst + v * 1024), "v"(off[v]), "v"(off[v + 1]), "v"(off[v + 2]), "v"(off[v + 3]), "s"(base) : "memory");
   }
 }

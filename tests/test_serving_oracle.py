@@ -145,3 +145,35 @@ def test_shape_functions():
         assert ops.kv_page_write_(e(7, 2, 64, dt=torch.bfloat16), e(7, 2, 64, dt=torch.bfloat16), kp, kp, slots) is None
         tok = ops.sample_tokens(e(5, 100, dt=torch.float32), e(5, dt=torch.float32))
         assert tok.shape == (5,) and tok.dtype == torch.int32
+
+
+def test_tracers_and_modes_see_the_operators():
+    """Eager calls on plain tensors do not go through the dispatcher; calls that something traces or intercepts do."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    logits, u = torch.zeros(2, 8), torch.zeros(2)
+    named = lambda gm: any("sample_tokens" in str(n.target) for n in gm.graph.nodes)
+    assert named(make_fx(lambda x, y: ops.sample_tokens(x, u=y), tracing_mode="fake")(logits, u))
+
+    seen = []
+
+    class See(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return torch.zeros(2, dtype=torch.int32) if "sample_tokens" in str(func) else func(*args, **(kwargs or {}))
+
+    with See():
+        ops.sample_tokens(logits, u)
+    assert any("sample_tokens" in s for s in seen)
+
+    with FakeTensorMode() as mode:
+        fake = torch.empty((2, 8)), torch.empty(2)
+    assert ops.sample_tokens(*fake).shape == (2,)             # outside of the mode that made them
+
+    graphs = []
+    compiled = torch.compile(lambda x, y: ops.sample_tokens(x, y) + 1, fullgraph=True,
+                             backend=lambda gm, _: graphs.append(gm) or gm.forward)
+    with pytest.raises(RuntimeError, match="GPU"):            # traced whole, then refused where it runs: on the CPU
+        compiled(logits, u)
+    assert named(graphs[0])
