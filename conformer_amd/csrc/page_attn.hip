@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
 // in flight or in use, K a tile ahead of V: the products for tile i + 1's scores stand beside tile i's exponentials.
 // Bound by the matrix and vector units together: at 128 head dims each is busy for about half of the time, and what one wave
 // needs of one the other wave of the SIMD must leave.  3 prompts of up to 8192 rows, 32 heads of 128 over 8, window 4096:
-// 0.88 ms, 1005 TFLOP/s in bf16, where a large matrix product reaches 1320; 85 in fp32 (143).
+// 0.86 ms, 1027 TFLOP/s in bf16, where a large matrix product reaches 1320; 85 in fp32 (143).
 //
 // C layout of a 32x32 product: lane (h = lane / 32, c = lane % 32), register i: row 8 (i / 4) + 4 h + i % 4, column c.  With
 // rows = tokens, registers 8 s .. 8 s + 7 are the eight tokens {4 h + 0..3, 8 + 4 h + 0..3} of 16-token step s: the k
