@@ -627,6 +627,7 @@ def _(enc_proj, pred_proj, out_w, out_b, d_joint, blank, max_symbols, clamp, cap
 # intercepts does not go through the dispatcher at all (10.5 against 9.5 us for that write, 14.1 against 12.1 for attention).
 _serving = torch.library.Library("fcenc", "FRAGMENT")
 _modes = torch._C._len_torch_dispatch_stack
+_transforms = torch._C._functorch.peek_interpreter_stack
 _plain = frozenset((Tensor, int, float, bool, type(None))).issuperset
 
 
@@ -642,8 +643,8 @@ def _serving_op(mutates: Tuple[str, ...] = ()):
 
         @functools.wraps(fn)
         def call(*args, **kwargs):
-            if (not torch.compiler.is_compiling() and _modes() == 0 and _plain(map(type, args))
-                    and (not kwargs or _plain(map(type, kwargs.values())))):
+            if (not torch.compiler.is_compiling() and _modes() == 0 and _transforms() is None
+                    and _plain(map(type, args)) and (not kwargs or _plain(map(type, kwargs.values())))):
                 return fn(*args, **kwargs)
             return op(*args, **kwargs)
 

@@ -428,6 +428,14 @@ def test_sampling_where_one_step_of_the_histogram_holds_too_many(dtype):
             assert got[r] == int(kept[int((run <= uu * run[-1]).sum())]), (r, kk, pp)
 
 
+def test_sampling_under_a_transform():
+    """A wrapped tensor goes through the dispatcher, which calls the operator slice by slice."""
+    g = torch.Generator().manual_seed(8)
+    x, u = torch.randn(3, 4, 50, generator=g).cuda(), torch.rand(4, generator=g).cuda()
+    got = torch.func.vmap(lambda r: ops.sample_tokens(r, u))(x)
+    assert torch.equal(got, torch.stack([ops.sample_tokens(r, u) for r in x]))
+
+
 def test_sampling_largest_vocabulary_and_strided_rows():
     n = 1 << 18
     assert _sample(torch.zeros(2, n), [0.5, 1 - 2.0 ** -24]) == [n // 2, n - 1]
