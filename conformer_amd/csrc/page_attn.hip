@@ -106,9 +106,9 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const
     // 64 candidates at a time, their lengths along with the last ones: one memory latency for up to 63 requests, two for up to
     // 4095
     const int lane = threadIdx.x & 63;
-    int hi = a.B + 1, k = 0, start = 0, length = 0;
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 63) >> 6;
+    int hi = a.B + 1, k = 0, start = 0, length = 0, step;
+    do {                                       // the last trip looks at neighbours, also where one candidate was left
+      step = (hi - lo + 63) >> 6;
       const int b = lo + lane * step;
       if (b <= a.B) start = clamp_rows(a.cu_rows[b], a.rows);
       if (step == 1 && b < a.B) length = a.kv_lens[b];
@@ -116,7 +116,7 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const
       k = k > 0 ? k : 0;
       lo = lo + k * step;
       hi = hi < lo + step ? hi : lo + step;
-    }
+    } while (step > 1);
     k = uniform(k);
     lo = uniform(lo);
     c0 = __builtin_amdgcn_readlane(start, k);

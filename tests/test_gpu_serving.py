@@ -154,10 +154,10 @@ def test_attention_extreme_windows_and_unit_dimensions():
     ops.kv_page_write_(k.as_strided((1, 1, 64), (1, 1, 1)), k, odd(kc), odd(vc), torch.tensor([16 * table[0][0] + 5]).cuda())
 
 
-@pytest.mark.parametrize("many", [70, 300, 4200])
+@pytest.mark.parametrize("many", [63, 64, 66, 70, 300, 4200, 4280])
 def test_attention_many_requests(many):
     """The search for a tile's request over more than 64 and more than 4096 of them, with empty ones among them."""
-    new = [(i * 7) % 3 if many < 1000 else int(i % 97 == 5) for i in range(many)]
+    new = [(i * 7) % 3 if many < 1000 else int(i % 97 == 5 or many > 4200) for i in range(many)]
     kv = [n + (i * 5) % 20 for i, n in enumerate(new)]
     q, kp, vp, table, cu = _problem(torch.bfloat16, 2, 1, 16, 16, new, kv, 9)
     _check(_run(q, kp, vp, table, kv, cu, 0.25), q, kp, vp, table, kv, cu, 0.25, torch.bfloat16)
