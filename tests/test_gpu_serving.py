@@ -228,14 +228,15 @@ def test_attention_and_write_past_32_bit_offsets():
     k, v = (torch.randn(kv, 1, d, generator=g).bfloat16() for _ in range(2))
     slots = torch.tensor([pages[j // ps] * ps + j % ps for j in range(kv)])
     ops.kv_page_write_(k.cuda(), v.cuda(), kp, vp, slots.cuda())
-    q = torch.randn(2, 4, d, generator=g).bfloat16()
+    q = torch.randn(60, 4, d, generator=g).bfloat16()
     i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
-    got = ops.kv_page_attention(q.cuda(), kp, vp, i32([pages]), i32([kv]), i32([0, 2]), 0.09)
     small = torch.zeros(3, 1, ps, d, dtype=torch.bfloat16), torch.zeros(3, 1, ps, d, dtype=torch.bfloat16)
     for t, src in zip(small, (k, v)):
         for j in range(kv):
             t[j // ps, 0, j % ps] = src[j, 0]
-    _check(got, q, *small, [[0, 1, 2]], [kv], [0, 2], 0.09, torch.bfloat16)
+    for n in (2, 60):                                          # the kernels of short chunks and of long ones
+        got = ops.kv_page_attention(q[:n].cuda(), kp, vp, i32([pages]), i32([kv]), i32([0, n]), 0.09)
+        _check(got, q[:n], *small, [[0, 1, 2]], [kv], [0, n], 0.09, torch.bfloat16)
 
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -610,6 +611,31 @@ def test_two_graphs_do_not_share_a_workspace():
     torch.cuda.synchronize()
     for i, r in enumerate(res):
         assert torch.equal(r, want[i % 2])
+
+
+def test_a_captured_chunk_call_follows_its_lengths():
+    """One captured call, replayed for batches in which the same requests bring single tokens, chunks, prompts or nothing: which kernel
+    takes a request and how its key axis is cut is found on the device."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    most = [1500, 900, 700, 1100]
+    q, kp, vp, table, _ = _problem(torch.bfloat16, 8, 2, 64, 32, [30, 30, 30, 30], most, 31)
+    kv, cu = i32(most), i32([0, 30, 60, 90, 120])
+    args = q.cuda(), kp.cuda(), vp.cuda(), i32(table), kv, cu, 0.125
+    ops.kv_page_attention(*args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.kv_page_attention(*args)
+    for new, lens in (([30, 30, 30, 30], most), ([1, 1, 1, 1], [1500, 1, 33, 1100]), ([90, 0, 1, 20], [90, 0, 700, 1100]),
+                      ([0, 0, 0, 0], [0, 0, 0, 0]), ([2, 100, 3, 15], [1400, 900, 3, 15])):
+        starts = [sum(new[:i]) for i in range(5)]
+        kv.copy_(i32(lens))
+        cu.copy_(i32(starts))
+        graph.replay()
+        assert torch.equal(got, ops.kv_page_attention(*args))
+        assert (got[starts[-1]:] == 0).all()
+        if starts[-1]:
+            _check(got[:starts[-1]], q[:starts[-1]], kp, vp, table, lens, starts, 0.125, torch.bfloat16)
 
 
 def test_refusals():
