@@ -664,7 +664,7 @@ def _no_grad(*operands: Tensor) -> None:
 
 def _on(t: Tensor, dev: int, dtype: torch.dtype, name: str, ndim: int) -> None:
     """An operand of the serving operators: on GPU `dev`, unit stride along its last dimension."""
-    if t.get_device() == dev >= 0 and t.dtype is dtype and t.dim() == ndim and (t.stride(-1) == 1 or t.shape[-1] <= 1):
+    if t.get_device() == dev >= 0 and t.dtype is dtype and t.dim() == ndim and (t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] <= 1):
         return
     if t.get_device() != dev or dev < 0:
         raise RuntimeError(f"fcenc: {name} must live on the GPU, beside the other operands (got {t.device})")
@@ -722,9 +722,9 @@ def kv_page_plan_(kv_lens: Tensor, new_lens: Tensor, finished: Optional[Tensor],
             raise ValueError("fcenc::kv_page_plan_: finished must hold one entry per table row")
     if rows < 0 or rows >= 2 ** 31 or b == 0 or w == 0 or free_pages.numel() == 0:
         raise ValueError(f"fcenc::kv_page_plan_: {rows} rows, table {b} x {w}, {free_pages.numel()} pages")
-    slots = torch.empty(rows, dtype=torch.int64, device=kv_lens.device)
-    cu_rows = torch.empty(b + 1, dtype=torch.int32, device=kv_lens.device)
-    granted = torch.empty(b, dtype=torch.bool, device=kv_lens.device)
+    slots = kv_lens.new_empty(rows, dtype=torch.int64)
+    cu_rows = kv_lens.new_empty(b + 1)
+    granted = kv_lens.new_empty(b, dtype=torch.bool)
     _launch(dev, N.lib().fcenc_page_plan, kv_lens.data_ptr(), new_lens.data_ptr(), N.ptr(finished), b, block_table.data_ptr(),
             block_table.stride(0) if b > 1 else w, w, free_pages.data_ptr(), free_count.data_ptr(), free_pages.numel(), page_size,
             slots.data_ptr(), rows, cu_rows.data_ptr(), granted.data_ptr())
@@ -789,14 +789,14 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
         raise ValueError(f"fcenc::kv_page_attention: q {tuple(q.shape)}, pages {tuple(k_pages.shape)}, {b} table rows, "
                          f"{kv_lens.numel()} lengths, {cu_rows.numel()} row offsets")
     dt = _cdt(q)
-    out = torch.empty(n, h, d, dtype=q.dtype, device=q.device)
+    out = q.new_empty((n, h, d))
     if n == 0:
         return out
     rows = N.PageRows(q.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), cu_rows.data_ptr(), q.stride(0), q.stride(1),
                       block_table.stride(0) if b > 1 else w, b, n, h, w, window, sinks, int(causal), max_rows, scale)
     lib = N.lib()
     need = lib.fcenc_page_attention_workspace_bytes(dt, C.byref(pages), C.byref(rows))
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     _launch(dev, lib.fcenc_page_attention, dt, C.byref(pages), C.byref(rows), out.data_ptr(), N.ptr(ws), need)
     return out
 
@@ -826,7 +826,7 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Optional[Tensor] = Non
                 raise ValueError(f"fcenc::sample_tokens: {nm} must hold one value per row")
     if v == 0:
         raise ValueError("fcenc::sample_tokens: empty vocabulary")
-    tokens = torch.empty(r, dtype=torch.int32, device=logits.device)
+    tokens = logits.new_empty(r, dtype=torch.int32)
     if r == 0:
         return tokens
     _launch(dev, N.lib().fcenc_sample_tokens, _cdt(logits), logits.data_ptr(), logits.stride(0) if r > 1 else v, r, v,
