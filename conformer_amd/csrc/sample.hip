@@ -761,7 +761,8 @@ __device__ __forceinline__ bool sample_by_value(char* smem, const RowSource<bf16
   const int top_i = (int)lds.word[0];
   if (lds.word[1] || top_i >= BV_LOW) return false;
   const float top = value_at(top_i);
-  if ((double)top + 128.0 < 40.0 * (double)t ? lds.count[BV_LOW] > 0 : false) return false;      // low values that weigh something
+  // low values that may matter: those of half a unit and more, and at u = 0 (or NaN) every weight that is a number at all
+  if ((double)top + 128.0 < (u > 0.f ? 40.0 : 745.14) * (double)t && lds.count[BV_LOW] > 0) return false;
   RowParams p;
   p.top = top;
   p.bins = 0.f;

@@ -402,6 +402,22 @@ def test_sampling_long_bf16_rows_at_the_ends_of_the_value_range(v):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [8192, 8193, 20000])
+def test_sampling_at_u_zero_takes_a_token_of_any_weight(dtype, v):
+    """u = 0 draws the first kept token whose weight is a number at all, also far below the units that sums are held in: logits at
+    and below -2^7 in front of a long row."""
+    x = torch.zeros(8, v)
+    x[:, 0] = torch.tensor([-200.0, -128.0, -744.0, -760.0, -math.inf, -200.0, -200.0, -300.0])
+    x[:, 1] = torch.tensor([0.0, 0.0, 0.0, -130.0, -700.0, 0.0, -150.0, -1.0])
+    x = x.to(dtype)
+    u = [0.0] * 8
+    for t, k, p, m in ((None, None, None, None), ([0.5] * 8, None, None, None), ([0.1] * 8, None, None, None), ([math.inf] * 8, None, None, None),
+                       (None, [v - 1] * 8, None, None), (None, None, [0.9] * 8, None), (None, None, None, [1e-30] * 8)):
+        assert _sample(x, u, t, k, p, m) == _want(x, u, t, k, p, m), (t, k, p, m)
+    assert _sample(x, u) == [0, 0, 0, 1, 1, 0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_sampling_where_one_step_of_the_histogram_holds_too_many(dtype):
     """Thousands of equal logits, and thousands within one step: the candidate list does not fit."""
     n = 1 << 15
