@@ -588,7 +588,7 @@ __device__ __forceinline__ int by_few(const SampleLds& lds, const RowParams& p, 
   const u64 wr = mine && tid < (int)k ? lds.mass[tid] : 0;   // of rank tid
   const u64 before = block_running(lds, wr, waves, total) - wr;
   const double target = (double)top_p * (double)total;
-  const bool in = mine && tid < (int)k && (top_p >= 1.f || (double)before < target || tid == 0);
+  const bool in = mine && tid < (int)k && (!(top_p < 1.f) || (double)before < target || tid == 0);
   // what top-k and top-p keep is a head of the ranks
   const u64 head = __ballot(in);
   __syncthreads();

@@ -418,6 +418,18 @@ def test_sampling_at_u_zero_takes_a_token_of_any_weight(dtype, v):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [50, 700, 9000])
+def test_sampling_filters_that_are_nan_are_off(dtype, v):
+    """In every form: few candidates and many, long rows and short ones."""
+    g = torch.Generator().manual_seed(v)
+    x = (torch.randn(8, v, generator=g) * 2).to(dtype)
+    u, nan = torch.rand(8, generator=g).tolist(), [math.nan] * 8
+    for k in (None, [40] * 8, [v // 2] * 8):
+        assert _sample(x, u, None, k, nan, nan) == _sample(x, u, None, k) == _want(x, u, None, k), k
+        assert _sample(x, u, nan, k) == _want(x, u, [0.0] * 8)           # a temperature that is not above 0: the first maximum
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_sampling_where_one_step_of_the_histogram_holds_too_many(dtype):
     """Thousands of equal logits, and thousands within one step: the candidate list does not fit."""
     n = 1 << 15
