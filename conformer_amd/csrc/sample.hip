@@ -816,12 +816,13 @@ __device__ __forceinline__ bool sample_by_value(char* smem, const RowSource<bf16
     u64 mm = mb;
 #pragma unroll
     for (int j = 0; j < BV_PER; ++j) {
-      if ((double)mm < target && target <= (double)(mm + cnt[j] * w[j])) publish(j, 0, mm);
+      if ((double)mm < target && target <= (double)(mm + cnt[j] * w[j])) publish(j, cnt[j], mm);
       mm += cnt[j] * w[j];
     }
     __syncthreads();
     const double r = ceil((target - (double)lds.mass[1]) / (double)lds.part_m[0]);      // kept while mass + i w < target
-    const unsigned rr = r < 1.0 ? 1u : (r > (double)MAX_VOCAB ? (unsigned)MAX_VOCAB : (unsigned)r);
+    // (sums are rounded to doubles here: r may come out above the number there is)
+    const unsigned rr = r < 1.0 ? 1u : (r > (double)lds.word[3] ? lds.word[3] : (unsigned)r);
     const int at = (int)lds.word[2];
     ties = at == border && rr > ties ? ties : rr;
     border = at;

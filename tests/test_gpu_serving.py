@@ -430,6 +430,18 @@ def test_sampling_filters_that_are_nan_are_off(dtype, v):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("second,low,tops,lows,p", [(-0.5, -9.0, 35104, 11445, 0.9999597668647766), (-0.5, -11.0, 52562, 57777, 0.9999816417694092),
+                                                    (-0.75, -9.0, 51295, 45541, 0.9998904466629028), (-1.5, -9.5, 48411, 14418, 0.999977707862854)])
+def test_sampling_where_top_p_ends_at_a_rounded_sum(dtype, second, low, tops, lows, p):
+    """`tops` logits of 0, one of `second`, `lows` of `low`: in units of 2^-46 the mass down to `second` passes 2^53, and p times the whole
+    mass, as a double, equals that sum rounded up.  The last token that has any part in the kept mass is `second`'s (the first low one
+    weighs less than 2^-24 of it)."""
+    x = torch.full((1, 131072), -math.inf)
+    x[0, :tops], x[0, tops], x[0, tops + 1:tops + 1 + lows] = 0.0, second, low
+    assert _sample(x.to(dtype), [1 - 2.0 ** -24], None, None, [p]) == [tops]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_sampling_where_one_step_of_the_histogram_holds_too_many(dtype):
     """Thousands of equal logits, and thousands within one step: the candidate list does not fit."""
     n = 1 << 15
