@@ -177,3 +177,36 @@ def test_tracers_and_modes_see_the_operators():
     with pytest.raises(RuntimeError, match="GPU"):            # traced whole, then refused where it runs: on the CPU
         compiled(logits, u)
     assert named(graphs[0])
+
+
+def _stand_in(name, mutates=()):
+    """An operator registered as the serving ones are, with a kernel that runs on the CPU and leaves nothing for a tracer to see."""
+    def put(to, x):
+        C.memmove(to.data_ptr(), (x.numpy(force=True) * 2).ctypes.data, 4 * x.numel())
+
+    if mutates:
+        def fn(x: torch.Tensor, y: torch.Tensor) -> None:
+            ops._no_grad(x, y)
+            put(y, x)
+    else:
+        def fn(x: torch.Tensor) -> torch.Tensor:
+            ops._no_grad(x)
+            y = x.new_empty(x.shape)
+            put(y, x)
+            return y
+    fn.__name__ = name
+    return ops._serving_op(mutates)(fn)
+
+
+def test_a_torchscript_trace_records_the_operators():
+    twice, twice_ = _stand_in("traced_twice"), _stand_in("traced_twice_", ("y",))
+    x = torch.arange(4.0)
+
+    def both(x):
+        y = torch.zeros_like(x)
+        twice_(x, y)
+        return twice(x), y
+
+    traced = torch.jit.trace(both, (x,), check_trace=False)
+    for got in traced(x + 1):
+        assert torch.equal(got, 2 * (x + 1))
