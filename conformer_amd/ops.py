@@ -629,6 +629,8 @@ _serving = torch.library.Library("fcenc", "FRAGMENT")
 _modes = torch._C._len_torch_dispatch_stack
 _transforms = torch._C._functorch.peek_interpreter_stack
 _tracer = torch._C._get_tracing_state
+_function_modes = torch._C._is_torch_function_mode_enabled
+_profiled = torch.autograd._profiler_enabled
 _plain = frozenset((Tensor, int, float, bool, type(None))).issuperset
 
 
@@ -645,7 +647,7 @@ def _serving_op(mutates: Tuple[str, ...] = ()):
         @functools.wraps(fn)
         def call(*args, **kwargs):
             if (not torch.compiler.is_compiling() and _modes() == 0 and _transforms() is None and _tracer() is None
-                    and _plain(map(type, args)) and (not kwargs or _plain(map(type, kwargs.values())))):
+                    and not _function_modes() and not _profiled() and _plain(map(type, args)) and (not kwargs or _plain(map(type, kwargs.values())))):
                 return fn(*args, **kwargs)
             return op(*args, **kwargs)
 

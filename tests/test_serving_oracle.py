@@ -210,3 +210,20 @@ def test_a_torchscript_trace_records_the_operators():
     traced = torch.jit.trace(both, (x,), check_trace=False)
     for got in traced(x + 1):
         assert torch.equal(got, 2 * (x + 1))
+
+
+def test_function_modes_and_profilers_see_the_operators():
+    from torch.overrides import TorchFunctionMode
+    twice, x, seen = _stand_in("seen_twice"), torch.arange(4.0), []
+
+    class See(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with See():
+        assert torch.equal(twice(x), 2 * x)
+    assert any("seen_twice" in s for s in seen)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
+        twice(x)
+    assert any("seen_twice" in e.key for e in prof.key_averages())
