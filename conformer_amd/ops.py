@@ -631,6 +631,7 @@ _transforms = torch._C._functorch.peek_interpreter_stack
 _tracer = torch._C._get_tracing_state
 _function_modes = torch._C._is_torch_function_mode_enabled
 _profiled = torch.autograd._profiler_enabled
+_forward_ad = torch.autograd.forward_ad
 _plain = frozenset((Tensor, int, float, bool, type(None))).issuperset
 
 
@@ -644,10 +645,17 @@ def _serving_op(mutates: Tuple[str, ...] = ()):
         op = getattr(torch.ops.fcenc, name).default
         op.__doc__ = fn.__doc__
 
+        def no_derivative(*args):
+            _no_grad(*(t for t in args if isinstance(t, Tensor)))
+            with torch._C._AutoDispatchBelowAutograd():
+                return op(*args)
+
+        _serving.impl(name, no_derivative, "Autograd")
+
         @functools.wraps(fn)
         def call(*args, **kwargs):
             if (not torch.compiler.is_compiling() and _modes() == 0 and _transforms() is None and _tracer() is None
-                    and not _function_modes() and not _profiled() and _plain(map(type, args)) and (not kwargs or _plain(map(type, kwargs.values())))):
+                    and not _function_modes() and not _profiled() and _forward_ad._current_level < 0 and _plain(map(type, args)) and (not kwargs or _plain(map(type, kwargs.values())))):
                 return fn(*args, **kwargs)
             return op(*args, **kwargs)
 
@@ -663,6 +671,8 @@ def _fake(call):
 def _no_grad(*operands: Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in operands):
         raise RuntimeError("fcenc: the serving operators have no backward pass; call them under torch.no_grad()")
+    if _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(t).tangent is not None for t in operands):
+        raise RuntimeError("fcenc: the serving operators have no forward-mode derivative")
 
 
 def _on(t: Tensor, dev: int, dtype: torch.dtype, name: str, ndim: int) -> None:

@@ -227,3 +227,30 @@ def test_function_modes_and_profilers_see_the_operators():
     with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CPU]) as prof:
         twice(x)
     assert any("seen_twice" in e.key for e in prof.key_averages())
+
+
+def test_derivatives_are_refused_not_dropped():
+    """Forward mode, and the transforms, whose tensors the kernels never meet as tensors that require a gradient."""
+    from torch.autograd import forward_ad
+    x, y = torch.arange(4.0), torch.zeros(4)
+    twice, twice_ = _stand_in("derived_twice"), _stand_in("derived_twice_", ("y",))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(4))
+        for call in (lambda: twice(dual), lambda: twice.op(dual), lambda: twice_(dual, y), lambda: twice_(x, forward_ad.make_dual(y, x))):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call()
+        assert torch.equal(twice(x), 2 * x)                   # an operand without a tangent
+    for call in (twice, twice.op):
+        with pytest.raises(RuntimeError, match="derivative"):
+            torch.func.jvp(call, (x,), (torch.ones(4),))
+        with pytest.raises(RuntimeError, match="backward"):
+            torch.func.grad(lambda x: call(x).sum())(x)
+        with pytest.raises(RuntimeError, match="backward"):
+            call(x.clone().requires_grad_())
+        with torch.no_grad():
+            assert torch.equal(call(x.clone().requires_grad_()), 2 * x)
+        assert torch.equal(torch.func.vmap(call)(torch.stack([x, x + 1])), 2 * torch.stack([x, x + 1]))
+        with torch.inference_mode():
+            assert torch.equal(call(x + 1), 2 * (x + 1))
+    # a transform over other operands
+    assert torch.equal(torch.func.grad(lambda a: (a * twice(x)).sum())(x), 2 * x)
