@@ -635,6 +635,10 @@ _forward_ad = torch.autograd.forward_ad
 _plain = frozenset((Tensor, int, float, bool, type(None))).issuperset
 
 
+class _Unresolved(Exception):
+    """An operand whose memory holds the negative of its values (the imaginary part of a conjugate): the dispatcher resolves it."""
+
+
 def _serving_op(mutates: Tuple[str, ...] = ()):
     """Registers a function as torch.ops.fcenc.<its name>.  The CPU entry is the same function: it refuses the operands."""
     def register(fn):
@@ -656,7 +660,10 @@ def _serving_op(mutates: Tuple[str, ...] = ()):
         def call(*args, **kwargs):
             if (not torch.compiler.is_compiling() and _modes() == 0 and _transforms() is None and _tracer() is None
                     and not _function_modes() and not _profiled() and _forward_ad._current_level < 0 and _plain(map(type, args)) and (not kwargs or _plain(map(type, kwargs.values())))):
-                return fn(*args, **kwargs)
+                try:
+                    return fn(*args, **kwargs)
+                except _Unresolved:
+                    pass
             return op(*args, **kwargs)
 
         call.op = op
@@ -678,6 +685,8 @@ def _no_grad(*operands: Tensor) -> None:
 def _on(t: Tensor, dev: int, dtype: torch.dtype, name: str, ndim: int) -> None:
     """An operand of the serving operators: on GPU `dev`, unit stride along its last dimension."""
     if t.get_device() == dev >= 0 and t.dtype is dtype and t.dim() == ndim and (t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] <= 1):
+        if dtype is torch.float32 and t.is_neg():
+            raise _Unresolved
         return
     if t.get_device() != dev or dev < 0:
         raise RuntimeError(f"fcenc: {name} must live on the GPU, beside the other operands (got {t.device})")

@@ -477,6 +477,16 @@ def test_sampling_under_a_transform():
     assert torch.equal(got, torch.stack([ops.sample_tokens(r, u) for r in x]))
 
 
+def test_lazily_negated_operands():
+    """The imaginary part of a conjugate is a view whose memory holds the negative of its values."""
+    u = torch.tensor([0.7j]).neg().cuda().conj().imag
+    assert u.is_neg() and abs(float(u) - 0.7) < 1e-6
+    row = torch.zeros(1, 10).cuda()
+    # ten equal weights; 0.7 in fp32 is 0.69999999, and 7 > 6.9999999: the seventh
+    assert ops.sample_tokens(row, u).tolist() == [6] == ops.sample_tokens.op(row, u).tolist()
+    assert ops.sample_tokens(row, u, temperature=u, min_p=u).tolist() == [6]
+
+
 def test_sampling_largest_vocabulary_and_strided_rows():
     n = 1 << 18
     assert _sample(torch.zeros(2, n), [0.5, 1 - 2.0 ** -24]) == [n // 2, n - 1]
