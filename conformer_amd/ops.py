@@ -697,6 +697,12 @@ def _on(t: Tensor, dev: int, dtype: torch.dtype, name: str, ndim: int) -> None:
     raise ValueError(f"fcenc: {name} must be contiguous along its last dimension")
 
 
+def _i32(*values: int) -> None:
+    """Sizes and integers that cross the C ABI as `int`, which would drop their upper bits without a word."""
+    if max(values) >= 2 ** 31 or min(values) < -2 ** 31:
+        raise ValueError(f"fcenc: sizes and integer arguments must fit 32 bits, got {values}")
+
+
 def _launch(dev: int, call, *args) -> None:
     """call(*args, the GPU's current stream) with GPU `dev` current: a kernel is launched on the device that is,
     whatever its stream belongs to."""
@@ -714,6 +720,7 @@ def _pages(k_pages: Tensor, v_pages: Tensor, dev: int, dt: torch.dtype) -> N.Pag
     _on(k_pages, dev, dt, "k_pages", 4)
     _on(v_pages, dev, dt, "v_pages", 4)
     n, h, ps, d = k_pages.shape
+    _i32(n, h, ps, d)
     if v_pages.shape != k_pages.shape:
         raise ValueError(f"fcenc: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} differ")
     ks, vs = k_pages.stride(), v_pages.stride()
@@ -729,6 +736,7 @@ def kv_page_plan_(kv_lens: Tensor, new_lens: Tensor, finished: Optional[Tensor],
     (slots int64 [rows], cu_rows int32 [B + 1], granted bool [B]).  A row is granted when its tokens fit the table and the step's
     rows and it needs no page, or the stack covers all that rows 0 .. b want: its pages move from the stack to the table and
     kv_lens grows.  Slots are page * page_size + offset; -1 for refused requests and rows that belong to nobody."""
+    _i32(page_size, rows)
     dev = kv_lens.get_device()
     _on(kv_lens, dev, torch.int32, "kv_lens", 1)
     _on(new_lens, dev, torch.int32, "new_lens", 1)
@@ -736,13 +744,14 @@ def kv_page_plan_(kv_lens: Tensor, new_lens: Tensor, finished: Optional[Tensor],
     _on(free_pages, dev, torch.int32, "free_pages", 1)
     _on(free_count, dev, torch.int32, "free_count", 1)
     b, w = block_table.shape
+    _i32(b, w, free_pages.numel())
     if kv_lens.numel() != b or new_lens.numel() != b or free_count.numel() != 1:
         raise ValueError("fcenc::kv_page_plan_: kv_lens and new_lens must hold one entry per table row, free_count one")
     if finished is not None:
         _on(finished, dev, torch.bool, "finished", 1)
         if finished.numel() != b:
             raise ValueError("fcenc::kv_page_plan_: finished must hold one entry per table row")
-    if rows < 0 or rows >= 2 ** 31 or b == 0 or w == 0 or free_pages.numel() == 0:
+    if rows < 0 or b == 0 or w == 0 or free_pages.numel() == 0:
         raise ValueError(f"fcenc::kv_page_plan_: {rows} rows, table {b} x {w}, {free_pages.numel()} pages")
     slots = kv_lens.new_empty(rows, dtype=torch.int64)
     cu_rows = kv_lens.new_empty(b + 1)
@@ -773,6 +782,7 @@ def kv_page_write_(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots
     _on(slots, dev, torch.int64, "slots", 1)
     pages = _pages(k_pages, v_pages, dev, k_pages.dtype)
     n = slots.numel()
+    _i32(n)
     if tuple(k.shape) != (n, pages.kv_heads, pages.head_dim) or v.shape != k.shape:
         raise ValueError(f"fcenc::kv_page_write_: k {tuple(k.shape)} and v {tuple(v.shape)} for {n} slots of {tuple(k_pages.shape)}")
     if n == 0:
@@ -798,6 +808,7 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
     are zeros.  Slots that no row of a chunk sees may hold anything; a NaN or infinity among the values (V) that some row sees
     may also reach rows of the same chunk that do not.  `max_rows` = the longest chunk, if the caller knows it (0: unknown): a
     hint for speed only."""
+    _i32(window, sinks, max_rows)
     dev = q.get_device()
     _no_grad(q, k_pages, v_pages)
     _on(q, dev, q.dtype, "q", 3)
@@ -807,6 +818,7 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
     _on(cu_rows, dev, torch.int32, "cu_rows", 1)
     n, h, d = q.shape
     b, w = block_table.shape
+    _i32(n, h, b, w)
     if d != pages.head_dim or kv_lens.numel() != b or cu_rows.numel() != b + 1:
         raise ValueError(f"fcenc::kv_page_attention: q {tuple(q.shape)}, pages {tuple(k_pages.shape)}, {b} table rows, "
                          f"{kv_lens.numel()} lengths, {cu_rows.numel()} row offsets")
@@ -841,6 +853,7 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Optional[Tensor] = Non
     _no_grad(logits)
     _on(logits, dev, logits.dtype, "logits", 2)
     r, v = logits.shape
+    _i32(r, v)
     for nm, t in (("u", u), ("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
         if t is not None:
             _on(t, dev, torch.int32 if nm == "top_k" else torch.float32, nm, 1)

@@ -254,3 +254,19 @@ def test_derivatives_are_refused_not_dropped():
             assert torch.equal(call(x + 1), 2 * (x + 1))
     # a transform over other operands
     assert torch.equal(torch.func.grad(lambda a: (a * twice(x)).sum())(x), 2 * x)
+
+
+def test_integers_past_32_bits_are_refused():
+    """They cross the C ABI as `int`: a window of 2^32 + 64 must not become one of 64."""
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    attn = lambda **k: ops.kv_page_attention(torch.zeros(1, 2, 64), torch.zeros(4, 2, 16, 64), torch.zeros(4, 2, 16, 64), i32(1, 4), i32(1), i32(2), 0.1, **k)
+    for big in (2 ** 31, 2 ** 32, 2 ** 32 + 64, -2 ** 32 + 5):
+        for name in ("window", "sinks", "max_rows"):
+            with pytest.raises(ValueError, match="32 bits"):
+                attn(**{name: big})
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.kv_page_plan_(i32(2), i32(2), None, i32(2, 4), i32(9), i32(1), big + 16, 2)
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.kv_page_plan_(i32(2), i32(2), None, i32(2, 4), i32(9), i32(1), 16, big + 2)
+    with pytest.raises(RuntimeError, match="GPU"):            # the largest that fit
+        attn(window=2 ** 31 - 1, sinks=2 ** 31 - 1, max_rows=2 ** 31 - 1)
