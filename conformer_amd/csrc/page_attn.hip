@@ -48,7 +48,8 @@ struct Split {
   int pieces = 1;                            // of the key axis, at most; the results of more than one go to the workspace from float `ws` on
   int piece = 1 << 30;                       // longest piece, in the kernel's blocks of tokens
   long long ws = 0;
-  long long ws_rows = 0;                     // (row, head) pairs there: all of them, or per_request rows of every request
+  long long ws_rows = 0;                     // (row, head) pairs there: of every row, or
+  bool by_request = false;                   // of per_request rows of every request (share 1, where that is less)
 };
 
 // Partial results of a split key axis: (m, l) of every (row, head, piece), then the unnormalised sums.
@@ -140,7 +141,7 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const
 
 // where the partial results of a (row of request b, head) lie
 __device__ __forceinline__ long long ws_row(const PageAttnArgs& a, const Split& sp, const TileInfo& ti, int row, int head) {
-  return (sp.share == 1 ? (long long)ti.b * sp.per_request + row : (long long)ti.c0 + row) * a.heads + head;
+  return (sp.by_request ? (long long)ti.b * sp.per_request + row : (long long)ti.c0 + row) * a.heads + head;
 }
 
 // V^T fragment of a [32 tokens][DP] tile in LDS: element j of lane (g, r) is V[token 16 (j >> 2) + 4 g + (j & 3)][dim 16 db + r]
@@ -922,7 +923,7 @@ __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : Chunk
 // The output row of row `wrow` of a launch's workspace and how many pieces its results are in; 0: it is written already.
 __device__ __forceinline__ int joined_pieces(const PageAttnArgs& a, const Split& sp, int wrow, int log, int& row) {
   TileInfo ti;
-  if (sp.share == 1) {
+  if (sp.by_request) {
     ti.b = wrow / sp.per_request;
     row = wrow - ti.b * sp.per_request;
     ti.c0 = clamp_rows(a.cu_rows[ti.b], a.rows);
@@ -945,7 +946,7 @@ __device__ __forceinline__ int joined_pieces(const PageAttnArgs& a, const Split&
     ti.b = lo;
     ti.c0 = clamp_rows(a.cu_rows[lo], a.rows);
     ti.n = clamp_rows(a.cu_rows[lo + 1], a.rows) - ti.c0;
-    if (row - ti.c0 >= ti.n || (sp.share == 2 && ti.n <= sp.per_request)) return 0;
+    if (row - ti.c0 >= ti.n || (sp.share != 0 && (ti.n <= sp.per_request) == (sp.share == 2))) return 0;
   }
   ti.t0 = (row - ti.c0) / sp.tt * sp.tt;
   const int cap = a.width << a.shift, kv = a.kv_lens[ti.b];
@@ -1105,7 +1106,9 @@ Plan make_plan(const PageAttnArgs& a) {
     const long long full = chunks ? 0 : (a.rows + s.tt - 1) / s.tt, some = a.rows < a.B ? a.rows : a.B;
     divide(a, s, (full > some ? full : some) * a.kv_heads * s.hchunks, 2048, STEP_BLOCK);
     s.piece = s.piece < 16 ? s.piece : 16;
-    s.ws_rows = (chunks ? (long long)a.B * few : (long long)a.rows) * a.heads;
+    // a large table with a small step must not pay for the rows that its requests do not bring
+    s.by_request = chunks && (long long)a.B * few < a.rows;
+    s.ws_rows = (s.by_request ? (long long)a.B * few : (long long)a.rows) * a.heads;
   }
   if (chunks) {
     Split& s = p.chunk;

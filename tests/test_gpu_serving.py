@@ -134,6 +134,19 @@ def test_attention_pieces_by_length(dtype, extra_width, mask):
     assert torch.equal(got, _run(q, kp, vp, table, kv, cu, 0.125, **mask))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("max_rows", [0, 40])
+def test_attention_small_step_of_a_large_table(dtype, max_rows):
+    """Few of many requests bring rows, short ones and chunks, all of them with a key axis that is cut."""
+    new, kv = [0] * 200, [0] * 200
+    for b, n, k in ((5, 1, 5000), (60, 40, 3000), (61, 2, 2000), (100, 4, 4100), (101, 5, 2500), (199, 1, 20)):
+        new[b], kv[b] = n, k
+    q, kp, vp, table, cu = _problem(dtype, 8, 1, 64, 32, new, kv, 37, tail=2, extra_width=100)
+    got = _run(q, kp, vp, table, kv, cu, 0.125, max_rows=max_rows)
+    assert (got[cu[-1]:] == 0).all()
+    _check(got[:cu[-1]], q[:cu[-1]], kp, vp, table, kv, cu, 0.125, dtype)
+
+
 def test_attention_extreme_windows_and_unit_dimensions():
     """A window of 2^31 - 1 tokens is none, also where rows in front of the request's start share a tile with others; strides of
     dimensions of one element are not looked at."""

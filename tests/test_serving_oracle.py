@@ -270,3 +270,18 @@ def test_integers_past_32_bits_are_refused():
             ops.kv_page_plan_(i32(2), i32(2), None, i32(2, 4), i32(9), i32(1), 16, big + 2)
     with pytest.raises(RuntimeError, match="GPU"):            # the largest that fit
         attn(window=2 ** 31 - 1, sinks=2 ** 31 - 1, max_rows=2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("batch,rows,max_rows", [(1024, 16, 12), (4096, 40, 40), (100000, 64, 50), (40, 40, 0), (40, 400, 30), (1, 4000, 0), (2000, 4000, 100)])
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (8, 8), (64, 1)])
+def test_attention_workspace_follows_the_rows_of_the_step(batch, rows, max_rows, heads, kv_heads):
+    """However long the table is: at most 256 pieces of the key axis of each (row, head), and no more than make 2560 workgroups of the
+    rows' tiles; twice, as short requests and chunks may both be cut."""
+    pages = N.Pages(4096, 4096, 64 * 128 * kv_heads, 64 * 128, 128, 64 * 128 * kv_heads, 64 * 128, 128, 1 << 20, 64, kv_heads, 128)
+    r = N.PageRows(4096, 4096, 4096, 4096, heads * 128, 128, 2048, batch, rows, heads, 2048, 0, 0, 1, max_rows, 0.1)
+    group = heads // kv_heads
+    some = min(batch, rows)                              # one tile per request with rows at the least that can be supposed
+    pieces = [min(256, max(1, 2560 // (n * kv_heads))) for n in (some, -(-rows * min(group, 128) // 128))]
+    pair = 128 * 4 + 8
+    need = N.lib().fcenc_page_attention_workspace_bytes(N.BF16, C.byref(pages), C.byref(r))
+    assert need <= rows * heads * sum(pieces) * pair + 64
