@@ -14,8 +14,10 @@
 //
 // A tile is a set of rows of one (request, kv head): `tt` neighbouring rows of the chunk times the gc query heads that
 // share the kv head, so that a key read once serves all of them.  Workgroup t finds its request without any table:
-// start(b) = cu_rows[b] / tt + b grows by at least ceil(n / tt) from one request to the next, so the request of t is
-// the last one with start(b) <= t, and rows / tt + B + 1 workgroups cover every batch.
+// start(b) = cu_rows[b] / tt + min(b, cu_rows[b]) grows by at least ceil(n / tt) over a request of n rows (n > 0: the second
+// term grows by one or more, the first by n / tt rounded down) and never falls, so the request of t is the last one
+// with start(b) <= t, and rows / tt + min(B, rows) + 1 workgroups cover every batch, however many requests bring nothing
+// (a table of 16384 requests of which 25 bring 64 rows, 32 heads of 128 over 8: 24 ms with B in place of min(B, rows)).
 //
 // Everything is computed transposed: S^T = K Q^T has the query row on the lane's column and tokens on the accumulator
 // rows, and those rows are, as they are, the k elements of the B operand of O^T = V^T P^T once the V fragment is read
@@ -49,11 +51,14 @@ struct Split {
   int piece = 1 << 30;                       // longest piece, in the kernel's blocks of tokens
   long long ws = 0;
   long long ws_rows = 0;                     // (row, head) pairs there: of every row, or
-  bool by_request = false;                   // of per_request rows of every request (share 1, where that is less)
+  bool by_request = false;                   // of per_request rows of every request (share 1, where that is less), which is then also how tiles go
 };
 
 // Partial results of a split key axis: (m, l) of every (row, head, piece), then the unnormalised sums.
 __device__ __host__ __forceinline__ long long ws_sums(long long rows, int pieces) { return (2 * rows * pieces + 3) & ~3ll; }
+
+// first tile of request b, whose rows begin at c0
+__device__ __forceinline__ int first_tile(int b, int c0, int tt) { return c0 / tt + (b < c0 ? b : c0); }
 
 struct TileInfo {
   int b, t0, n, c0, kv;                      // request (B: rows behind the last one), first row, rows, offset, tokens
@@ -96,13 +101,13 @@ __device__ __forceinline__ int clamp_rows(int v, int rows) { return v < 0 ? 0 : 
 __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const Split& sp, TileInfo& ti) {
   const int tt = sp.tt;
   int lo = 0, c0, c1, kv;
-  if (sp.share == 1) {                         // as many tiles for every request
+  if (sp.by_request) {                         // as many tiles for every request
     const int each = (sp.per_request + tt - 1) / tt;
     lo = tile / each;
     c0 = clamp_rows(uniform(a.cu_rows[lo]), a.rows);
     c1 = clamp_rows(uniform(a.cu_rows[lo + 1]), a.rows);
     kv = uniform(a.kv_lens[lo]);
-    tile = tile - lo * each + c0 / tt + lo;
+    tile = tile - lo * each + first_tile(lo, c0, tt);
   } else {
     // 64 candidates at a time, their lengths along with the last ones: one memory latency for up to 63 requests, two for up to
     // 4095
@@ -113,7 +118,7 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const
       const int b = lo + lane * step;
       if (b <= a.B) start = clamp_rows(a.cu_rows[b], a.rows);
       if (step == 1 && b < a.B) length = a.kv_lens[b];
-      k = __popcll(__ballot(b < hi && start / tt + b <= tile)) - 1;     // starts rise with b
+      k = __popcll(__ballot(b < hi && first_tile(b, start, tt) <= tile)) - 1;     // starts rise with b
       k = k > 0 ? k : 0;
       lo = lo + k * step;
       hi = hi < lo + step ? hi : lo + step;
@@ -127,7 +132,7 @@ __device__ __forceinline__ bool find_tile(const PageAttnArgs& a, int tile, const
   ti.b = lo;
   ti.c0 = c0;
   ti.n = c1 - c0;
-  ti.t0 = (tile - (c0 / tt + lo)) * tt;
+  ti.t0 = (tile - first_tile(lo, c0, tt)) * tt;
   ti.kv = 0;
   if (ti.t0 < 0 || ti.t0 >= ti.n) return false;
   if (sp.share == 1 && ti.n > sp.per_request) return false;
@@ -1095,6 +1100,7 @@ Plan make_plan(const PageAttnArgs& a) {
   const long long longest = a.max_rows > 0 && a.max_rows < a.rows ? a.max_rows : a.rows;      // rows of one request
   // without a hint a batch of as many rows as requests is taken for single tokens
   const bool chunks = longest > few && (a.max_rows > 0 || a.rows > a.B || few == 0);
+  const long long some = a.rows < a.B ? a.rows : a.B;                                         // requests with rows, at most
   if (few > 0 || !chunks) {
     Split& s = p.step;
     s.gc = group < STEP_ROWS ? group : STEP_ROWS;
@@ -1102,12 +1108,12 @@ Plan make_plan(const PageAttnArgs& a) {
     s.tt = STEP_ROWS / s.gc;
     s.share = chunks ? 1 : 0;
     s.per_request = chunks ? few : 0;
-    p.step_tiles = chunks ? (long long)a.B * ((few + s.tt - 1) / s.tt) : (long long)a.rows / s.tt + a.B + 1;
-    const long long full = chunks ? 0 : (a.rows + s.tt - 1) / s.tt, some = a.rows < a.B ? a.rows : a.B;
+    const long long full = chunks ? 0 : (a.rows + s.tt - 1) / s.tt;
     divide(a, s, (full > some ? full : some) * a.kv_heads * s.hchunks, 2048, STEP_BLOCK);
     s.piece = s.piece < 16 ? s.piece : 16;
     // a large table with a small step must not pay for the rows that its requests do not bring
     s.by_request = chunks && (long long)a.B * few < a.rows;
+    p.step_tiles = s.by_request ? (long long)a.B * ((few + s.tt - 1) / s.tt) : (long long)a.rows / s.tt + some + 1;
     s.ws_rows = (s.by_request ? (long long)a.B * few : (long long)a.rows) * a.heads;
   }
   if (chunks) {
@@ -1117,7 +1123,7 @@ Plan make_plan(const PageAttnArgs& a) {
     s.tt = CHUNK_ROWS / s.gc;
     s.share = 2;
     s.per_request = few;
-    p.chunk_tiles = (long long)a.rows / s.tt + a.B + 1;
+    p.chunk_tiles = (long long)a.rows / s.tt + some + 1;
     divide(a, s, (long long)(a.rows + s.tt - 1) / s.tt * a.kv_heads * s.hchunks, 2560, CHUNK_BLOCK);
     s.ws_rows = (long long)a.rows * a.heads;
     s.ws = (ws_floats(a, p.step) + 3) & ~3ll;

@@ -147,6 +147,30 @@ def test_attention_small_step_of_a_large_table(dtype, max_rows):
     _check(got[:cu[-1]], q[:cu[-1]], kp, vp, table, kv, cu, 0.125, dtype)
 
 
+@pytest.mark.parametrize("longest", [1, 40])
+def test_attention_time_follows_the_rows_not_the_table(longest):
+    """The same 64 rows in a table of 64 requests and in one of 16384, where workgroups for every request would take 20 ms."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()
+    kp = torch.randn(64, 8, 64, 128, device="cuda").bfloat16()
+    q = torch.randn(64, 32, 128, device="cuda").bfloat16()
+    times = []
+    for batch in (64, 16384):
+        new, kv = [0] * batch, [0] * batch
+        for i in range(64 - longest + 1):
+            new[i], kv[i] = (longest, 2000) if i == 3 else (1, 500)
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + n)
+        args = q, kp, kp, torch.randint(0, 64, (batch, 512), dtype=torch.int32).cuda(), i32(kv), i32(cu), 0.09, 0, 0, True, longest
+        marks = [torch.cuda.Event(enable_timing=True) for _ in range(8)]
+        for m in marks:
+            ops.kv_page_attention(*args)
+            m.record()
+        torch.cuda.synchronize()
+        times.append(min(a.elapsed_time(b) for a, b in zip(marks, marks[1:])))
+    assert times[1] < 5 * times[0] + 0.1, times
+
+
 def test_attention_extreme_windows_and_unit_dimensions():
     """A window of 2^31 - 1 tokens is none, also where rows in front of the request's start share a tile with others; strides of
     dimensions of one element are not looked at."""
