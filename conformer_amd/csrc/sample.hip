@@ -61,35 +61,39 @@ __device__ constexpr ExpTable exp_table{};
 
 struct SampleLds {
   u64* mass;                 // [bins]
-  u64* part_m;               // [waves]
+  unsigned* count;           // [bins], also read in fours: at a multiple of 16 bytes
   double* table;             // [TABLE]
-  unsigned* count;           // [bins]
-  unsigned* part_c;          // [waves]
-  unsigned* seg_n;           // [waves] list entries
   float* seg_x;              // [waves][SEG]
   int* seg_i;                // [waves][SEG]
-  unsigned* lo;              // range of keys: lo, hi
+  u64* part_m;               // [waves]
   u64* found_m;              // a border found in the bins: mass before it,
   unsigned* found;           //   bin, count before it; [2]: a token index
+  unsigned* part_c;          // [waves]
+  unsigned* seg_n;           // [waves] list entries
+  unsigned* lo;              // range of keys: lo, hi
 };
 __host__ __device__ constexpr int lds_bytes(int waves) {
   return waves * BINS_PER_WAVE * 12 + waves * (8 + 4 + 4) + TABLE * 8 + waves * SEG * 8 + 8 + 8 + 16;
 }
+__host__ __device__ constexpr int count_at(int waves) { return waves * BINS_PER_WAVE * 8; }
+static_assert(count_at(1) % 16 == 0 && count_at(2) % 16 == 0 && count_at(4) % 16 == 0 && count_at(8) % 16 == 0 && count_at(16) % 16 == 0,
+              "by_few loads four counts at a time");
 
 __device__ __forceinline__ SampleLds carve(char* p, int waves) {
   SampleLds l;
-  auto take = [&](int bytes) { char* at = p; p += bytes; return at; };
-  l.mass = reinterpret_cast<u64*>(take(waves * BINS_PER_WAVE * 8));
-  l.part_m = reinterpret_cast<u64*>(take(waves * 8));
-  l.table = reinterpret_cast<double*>(take(TABLE * 8));
-  l.found_m = reinterpret_cast<u64*>(take(8));
+  char* at = p + count_at(waves);
+  auto take = [&](int bytes) { char* q = at; at += bytes; return q; };
+  l.mass = reinterpret_cast<u64*>(p);
   l.count = reinterpret_cast<unsigned*>(take(waves * BINS_PER_WAVE * 4));
-  l.part_c = reinterpret_cast<unsigned*>(take(waves * 4));
-  l.seg_n = reinterpret_cast<unsigned*>(take(waves * 4));
+  l.table = reinterpret_cast<double*>(take(TABLE * 8));
   l.seg_x = reinterpret_cast<float*>(take(waves * SEG * 4));
   l.seg_i = reinterpret_cast<int*>(take(waves * SEG * 4));
-  l.lo = reinterpret_cast<unsigned*>(take(8));
+  l.part_m = reinterpret_cast<u64*>(take(waves * 8));
+  l.found_m = reinterpret_cast<u64*>(take(8));
   l.found = reinterpret_cast<unsigned*>(take(16));
+  l.part_c = reinterpret_cast<unsigned*>(take(waves * 4));
+  l.seg_n = reinterpret_cast<unsigned*>(take(waves * 4));
+  l.lo = reinterpret_cast<unsigned*>(take(8));
   return l;
 }
 
