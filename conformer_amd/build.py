@@ -23,9 +23,9 @@ SOURCES = ["api.hip", "gemm.hip", "conv256.hip", "conv12.hip", "conv3p.hip", "ff
 # of their forms have given wrong results now and then.  (The host pass does not know the feature and says so; harmless.)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-Wall",
          "-Wno-unused-function", "-Wno-unused-variable", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# per-file additions.  elementwise.hip: conv1 is paced by the SiLU of its 655 M outputs; -O3 packs pairs of its fp32
-# multiplies into v_pk_mul_f32, which issue slower than the two scalar instructions they replace (measured on
-# MI355X: 280.5 -> 275.6 us with the packing off, same bits); the block kernels measured no difference.
+# per-file additions.  Without packed fp32 instructions -O3 still groups neighbouring scalar code of these files in its own way.
+# elementwise.hip: conv1 is paced by the SiLU of its 655 M outputs, and was faster without the grouping while that still formed
+# v_pk_mul_f32 (280.5 -> 275.6 us on MI355X, same bits); the block kernels measured no difference.
 EXTRA_FLAGS = {"elementwise.hip": ["-fno-slp-vectorize"], "conv12.hip": ["-fno-slp-vectorize"], "conv3p.hip": ["-fno-slp-vectorize"]}
 
 
@@ -43,17 +43,29 @@ def _stale(target: str, deps) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _commands(hipcc: str):
+    """(source, object, command) of every file."""
+    for src in SOURCES:
+        s, o = os.path.join(CSRC, src), os.path.join(OBJ, src.replace(".hip", ".o"))
+        yield s, o, [hipcc, *FLAGS, *EXTRA_FLAGS.get(src, []), "-c", s, "-o", o]
+
+
+def _built_with(o: str):
+    """The command that made an object, None if that is not known."""
+    try:
+        with open(o + ".cmd") as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def build_native(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     hipcc = _hipcc()
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     headers.append(os.path.join(os.path.dirname(HERE), "include", "fcenc.h"))
-    jobs = []
-    for src in SOURCES:
-        s = os.path.join(CSRC, src)
-        o = os.path.join(OBJ, src.replace(".hip", ".o"))
-        if force or _stale(o, [s] + headers):
-            jobs.append([hipcc, *FLAGS, *EXTRA_FLAGS.get(src, []), "-c", s, "-o", o])
+    # an object is as old as its sources and its command: changed flags make it again too
+    jobs = [(o, cmd) for s, o, cmd in _commands(hipcc) if force or _stale(o, [s] + headers) or _built_with(o) != " ".join(cmd)]
 
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
@@ -62,8 +74,14 @@ def build_native(force: bool = False, verbose: bool = False) -> str:
         if verbose and r.stderr.strip():
             print(r.stderr, file=sys.stderr)
 
+    def compile_one(job):
+        o, cmd = job
+        run(cmd)
+        with open(o + ".cmd", "w") as f:
+            f.write(" ".join(cmd))
+
     with ThreadPoolExecutor(max_workers=4) as ex:
-        list(ex.map(run, jobs))
+        list(ex.map(compile_one, jobs))
     objs = [os.path.join(OBJ, s.replace(".hip", ".o")) for s in SOURCES]
     if force or jobs or _stale(LIB, objs):
         run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", LIB])
