@@ -50,3 +50,11 @@ def test_changed_sources_compile_again(tree):
     assert sum("a.hip" in c for c in tree()) == 1
     os.utime(tree.csrc / "a.hip", (1, 1))
     assert len(tree(force=True)) == 3
+
+
+def test_the_entry_point_always_compiles(monkeypatch):
+    import __graft_entry__
+    seen = []
+    monkeypatch.setattr(build, "build_native", lambda **k: seen.append(k) or build.LIB)
+    __graft_entry__.build()
+    assert seen == [{"force": True}]
