@@ -9,8 +9,11 @@
 //
 // One pass over the keys with a running maximum m and sum l per row (fp32, base-2 exponents):
 //     m' = max(m, max_j s_j),  l' = l 2^(m - m') + sum_j 2^(s_j - m'),  O' = O 2^(m - m') + sum_j 2^(s_j - m') v_j.
-// In bf16 the p_j = 2^(s_j - m') are rounded for the product with v, and l adds up the rounded ones: what is rounded off in
-// the numerator is then missing in the denominator too, and a row that one key dominates loses nothing.
+// In bf16 p_j = 2^(s_j - m') has to be given to the product with v in bf16.  The kernel of short requests, bound by the bytes of K
+// and V, takes it as a sum of two bf16 numbers (good to 2^-15; 64 requests of up to 8192 tokens 257.1 us, 257.4 rounded
+// once).  The kernel of chunks and prompts, where a second product for every one of v would be half as much matrix work again,
+// rounds it once, and l adds up the rounded ones: what is rounded off in the numerator is then missing in the
+// denominator too, and a row that one key dominates loses nothing.
 //
 // A tile is a set of rows of one (request, kv head): `tt` neighbouring rows of the chunk times the gc query heads that
 // share the kv head, so that a key read once serves all of them.  Workgroup t finds its request without any table:
@@ -192,17 +195,7 @@ __device__ __forceinline__ f32x8 p_frag(const float (&x)[8], float) {
   return f;
 }
 
-// sum of a fragment's eight elements, as they are stored, on top of l
-__device__ __forceinline__ float add_frag(float l, const bf16x8& f) {
-  const u32x4 u = __builtin_bit_cast(u32x4, f);
-  float a = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    l += __builtin_bit_cast(float, u[i] << 16);
-    a += __builtin_bit_cast(float, u[i] & 0xffff0000u);
-  }
-  return l + a;
-}
+// sum of a fragment's eight elements on top of l
 __device__ __forceinline__ float add_frag(float l, const f32x8& f) {
   return l + (((f.lo[0] + f.lo[1]) + (f.lo[2] + f.lo[3])) + ((f.hi[0] + f.hi[1]) + (f.hi[2] + f.hi[3])));
 }
@@ -390,12 +383,26 @@ __device__ __forceinline__ void step_tile(const PageAttnArgs& a, const Split& sp
     float pk[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) pk[e] = __builtin_amdgcn_exp2f(st[e >> 2][e & 3] - m_use);
-    const Frag pf = p_frag(pk, T{});
-    l_run = add_frag(l_run * alpha, pf);
+    l_run = l_run * alpha + (((pk[0] + pk[1]) + (pk[2] + pk[3])) + ((pk[4] + pk[5]) + (pk[6] + pk[7])));
+    // bf16: p as the sum of two bf16 numbers.  The first is the largest one below p, so that the second is above 0 as well, and
+    // an infinite v gives infinity as it does with p itself; 0 stays 0.
+    float ph[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ph[e] = pk[e];
+      if constexpr (sizeof(T) == 2) {
+        const int below = __builtin_bit_cast(int, pk[e]) - 1;
+        ph[e] = __builtin_bit_cast(float, (below > 0 ? below : 0) & 0xffff0000);
+        pk[e] -= ph[e];
+      }
+    }
+    const Frag pf = p_frag(ph, T{}), pr = p_frag(pk, T{});
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       ot[db] *= alpha;
-      mma(ot[db], v_frag<ROWB>(vt, db, g, r, T{}), pf);
+      const Frag vf = v_frag<ROWB>(vt, db, g, r, T{});
+      mma(ot[db], vf, pf);
+      if constexpr (sizeof(T) == 2) mma(ot[db], vf, pr);
     }
   }
 

@@ -807,7 +807,8 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
     (not causal or j <= p) and (window == 0 or j > p - window or j < sinks).  Rows that see nothing, or belong to no request,
     are zeros.  Slots that no row of a chunk sees may hold anything; a NaN or infinity among the values (V) that some row sees
     may also reach rows of the same chunk that do not.  `max_rows` = the longest chunk, if the caller knows it (0: unknown): a
-    hint for speed only."""
+    hint for speed, which changes no more than roundings.  Scores, maxima and sums are fp32.  In bf16 the probabilities go into the product
+    with V as bf16: two numbers each (2^-15) where request and kv head have up to 32 rows x heads, one (2^-8) in longer chunks."""
     _i32(window, sinks, max_rows)
     dev = q.get_device()
     _no_grad(q, k_pages, v_pages)

@@ -480,8 +480,10 @@ int fcenc_mel_spectrogram(const fcenc_mel_plan* plan, const float* wave, long lo
  * that some row of the chunk sees, a key that is NaN or infinite reaches the rows that see it; a value (V) that is may also
  * reach rows of the same request and chunk that do not.  head_dim <= 128 and a multiple of 8; all strides in elements,
  * multiples of 16 bytes, of a page below 2^32 bytes; page_size slots of a head span at most 2 GiB; scale > 0.  max_rows: the
- * longest chunk of the batch if the caller knows it, else 0 -- it chooses kernels and never changes what is computed.  The
- * workspace (size from fcenc_page_attention_workspace_bytes, may be 0) belongs to one call at a time.
+ * longest chunk of the batch if the caller knows it, else 0 -- it chooses kernels, which changes no more than roundings.  Scores,
+ * maxima and sums are fp32; in bf16 the probabilities go into the product with V as bf16, two numbers each (good to 2^-15) for
+ * requests of up to 32 rows x heads per kv head, one (2^-8) in longer chunks.  The workspace (size from
+ * fcenc_page_attention_workspace_bytes, may be 0) belongs to one call at a time.
  *
  * fcenc_sample_tokens: one token per row of logits [rows][row_stride] (vocab <= 2^18 used).  With weights
  * w_i = exp((x_i - max) / temperature) and the order of falling logits (equal ones by rising index): top_k keeps the

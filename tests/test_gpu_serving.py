@@ -171,6 +171,33 @@ def test_attention_time_follows_the_rows_not_the_table(longest):
     assert times[1] < 5 * times[0] + 0.1, times
 
 
+@pytest.mark.parametrize("h,hk,d", [(8, 2, 128), (4, 4, 64), (3, 1, 40), (32, 1, 96)])
+@pytest.mark.parametrize("mask", [dict(), dict(window=30, sinks=3)])
+def test_attention_of_single_tokens_keeps_the_probabilities(h, hk, d, mask):
+    """Up to 32 rows times heads per kv head in bf16: the p_j are two bf16 numbers each, the first off by less than a whole step (2^-7),
+    the second, that difference, by half a step of it: 2^-15 before the last rounding instead of 2^-8."""
+    new, kv = [1, 1, 1, 1, 1], [2, 33, 70, 900, 2100]
+    q, kp, vp, table, cu = _problem(torch.bfloat16, h, hk, d, 32, new, kv, 41)
+    got = _run(q, kp, vp, table, kv, cu, d ** -0.5, **mask)
+    fin = lambda t: torch.nan_to_num(t.float(), nan=0.0)
+    want, mag = S.page_attention(q, kp, vp, table, kv, cu, d ** -0.5, **mask)
+    qk = fin(q).norm(dim=2).max() * fin(kp).norm(dim=3).max() * d ** -0.5
+    p_err = (d + 2) * 2.0 ** -24 * qk + 2.0 ** -22 * (qk + 1)
+    tol = mag * (2 * p_err + 2.0 ** -15 + 2 * max(kv) * 2.0 ** -24) + 2.0 ** -8 * want.abs() + 1e-30
+    err = (got.cpu().double() - want).abs()
+    assert (err <= tol).all(), (err / tol).max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kv", [50, 2500])
+def test_attention_of_single_tokens_keeps_infinite_values(dtype, kv):
+    q, kp, vp, table, cu = _problem(dtype, 4, 2, 64, 32, [1], [kv], 43)
+    want = _run(q, kp, vp, table, [kv], cu, 0.125)
+    vp[table[0][1], 0, 2, 5], vp[table[0][0], 1, 7, 60] = math.inf, -math.inf
+    want[0, :2, 5], want[0, 2:, 60] = math.inf, -math.inf
+    assert torch.equal(_run(q, kp, vp, table, [kv], cu, 0.125), want)
+
+
 def test_attention_extreme_windows_and_unit_dimensions():
     """A window of 2^31 - 1 tokens is none, also where rows in front of the request's start share a tile with others; strides of
     dimensions of one element are not looked at."""
