@@ -685,10 +685,12 @@ def _no_grad(*operands: Tensor) -> None:
 
 
 def _on(t: Tensor, dev: int, dtype: torch.dtype, name: str, ndim: int) -> None:
-    """An operand of the serving operators: on GPU `dev`, unit stride along its last dimension."""
+    """An operand of the serving operators: on GPU `dev`, unit stride along its last dimension, no gradient asked for."""
     if t.get_device() == dev >= 0 and t.dtype is dtype and t.dim() == ndim and (t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] <= 1):
         if dtype is torch.float32 and t.is_neg():
             raise _Unresolved
+        if t.requires_grad:
+            _no_grad(t)
         return
     if t.get_device() != dev or dev < 0:
         raise RuntimeError(f"fcenc: {name} must live on the GPU, beside the other operands (got {t.device})")
@@ -782,7 +784,6 @@ def kv_page_write_(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, slots
     slots int64 [N]; a slot outside the pool (-1) is skipped.  Slots must differ: of two rows with one slot either may
     stay."""
     dev = k_pages.get_device()
-    _no_grad(k, v, k_pages, v_pages)
     _on(k, dev, k_pages.dtype, "k", 3)
     _on(v, dev, k_pages.dtype, "v", 3)
     _on(slots, dev, torch.int64, "slots", 1)
@@ -819,7 +820,6 @@ def kv_page_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: 
     if (window | sinks | max_rows) >> 31:
         _past_32_bits(window, sinks, max_rows)
     dev = q.get_device()
-    _no_grad(q, k_pages, v_pages)
     _on(q, dev, q.dtype, "q", 3)
     pages = _pages(k_pages, v_pages, dev, q.dtype)
     _on(block_table, dev, torch.int32, "block_table", 2)
@@ -860,7 +860,6 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Optional[Tensor] = Non
     The token is the first one, in index order, whose running mass exceeds u times the kept mass.  temperature <= 0
     takes the first maximum.  NaN logits count as -inf; a row without any other gives -1."""
     dev = logits.get_device()
-    _no_grad(logits)
     _on(logits, dev, logits.dtype, "logits", 2)
     r, v = logits.shape
     if (r | v) >> 31:

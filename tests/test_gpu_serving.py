@@ -793,3 +793,21 @@ def test_refusals():
     assert ops.sample_tokens(x[:0], u[:0]).shape == (0,)
     with torch.no_grad():
         assert ops.sample_tokens(x.clone().requires_grad_(), u).tolist() == [0, 0]
+
+
+def test_operands_that_require_a_gradient_are_refused_wherever_they_stand():
+    x, u = torch.zeros(2, 9).cuda(), torch.full((2,), 0.5).cuda()
+    t = torch.ones(2).cuda().requires_grad_()
+    for call in (ops.sample_tokens, ops.sample_tokens.op):
+        for args in ((x, t), (x, u, t), (x, u, None, None, t), (x, u, None, None, None, t), (x.clone().requires_grad_(), u)):
+            with pytest.raises(RuntimeError, match="backward"):
+                call(*args)
+            with torch.no_grad():
+                call(*args)
+        assert call(x, u).tolist() == [4, 4]
+    pages = torch.zeros(2, 1, 16, 8).cuda()
+    k, slots = torch.ones(1, 1, 8).cuda(), torch.zeros(1, dtype=torch.int64).cuda()
+    for call in (ops.kv_page_write_, ops.kv_page_write_.op):
+        for args in ((k.clone().requires_grad_(), k, pages, pages, slots), (k, k, pages, pages.clone().requires_grad_(), slots)):
+            with pytest.raises(RuntimeError, match="backward"):
+                call(*args)
