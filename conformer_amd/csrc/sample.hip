@@ -10,7 +10,9 @@
 //
 // A token is a comparison of a sum with a border, so sums must not depend on the order of their terms: weights are
 // formed in fp64 and rounded to integers in units of 2^-b, b = min(51, 63 - ceil(log2 vocab)), so that no sum passes
-// 2^63, and integers add up exactly in any order, LDS atomics included.  A weight below half a unit counts as 0.
+// 2^63, and integers add up exactly in any order, LDS atomics included.  A weight below half a unit (2^-52 of the largest one up to 4096
+// logits, 2^-46 at the most there can be) counts as 0 and can be drawn only at u = 0, which takes the first kept token whose
+// weight is a number at all (as a double: (max - x) / t < 745.13).  A filter that is NaN is off; a temperature that is takes the maximum.
 //
 // One workgroup per row; a wave takes a contiguous piece of it.  The head's last token is found by counting, not
 // sorting: a histogram (counts or masses) over equal steps of (max - x) / t gives the step it lies in, histograms over

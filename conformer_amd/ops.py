@@ -858,7 +858,8 @@ def sample_tokens(logits: Tensor, u: Tensor, temperature: Optional[Tensor] = Non
     keeps the first k (<= 0: all), top_p fp32 [R] a token while the mass before it is below top_p times what top_k left
     (>= 1: all), min_p fp32 [R] those of at least min_p times the largest weight (<= 0: all); the first is always kept.
     The token is the first one, in index order, whose running mass exceeds u times the kept mass.  temperature <= 0
-    takes the first maximum.  NaN logits count as -inf; a row without any other gives -1."""
+    takes the first maximum.  NaN logits count as -inf; a row without any other gives -1.  Weights are formed in fp64 (to 1.4e-13) and
+    added up as integers in units of 2^-min(51, 63 - ceil(log2 V)): a weight below half a unit is drawn at u = 0 only."""
     dev = logits.get_device()
     _on(logits, dev, logits.dtype, "logits", 2)
     r, v = logits.shape

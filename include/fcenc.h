@@ -490,7 +490,9 @@ int fcenc_mel_spectrogram(const fcenc_mel_plan* plan, const float* wave, long lo
  * first k (<= 0: all), top_p keeps a token while the mass before it is below top_p times what top_k left (>= 1:
  * all), min_p keeps w_i >= min_p; the first is always kept.  u in [0, 1) picks, in index order, the first token whose
  * running sum exceeds u times the sum.  temperature <= 0: the first maximum.  NaN logits count as -inf; a row of
- * nothing but -inf gives -1.  Parameters are per row; null pointers mean temperature 1 and no filter. */
+ * nothing but -inf gives -1.  Parameters are per row; null pointers mean temperature 1 and no filter.  Weights are formed in fp64 (to
+ * 1.4e-13) and added up as integers in units of 2^-min(51, 63 - ceil(log2 vocab)): a weight below half a unit is drawn at u = 0
+ * only, which takes the first kept token whose weight is not 0 as a double. */
 typedef struct fcenc_pages {
   void* k;
   void* v;
