@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(64 * STEP_WAVES, (StepTile<T, DP>::ROWB > 256 
 // in flight or in use, K a tile ahead of V: the products for tile i + 1's scores stand beside tile i's exponentials.
 // Bound by the matrix and vector units together: at 128 head dims they are busy 57 and 49 % of the cycles, and what one wave
 // needs of one the other wave of the SIMD must leave.  3 prompts of up to 8192 rows, 32 heads of 128 over 8, window 4096:
-// 0.86 ms, 1027 TFLOP/s in bf16, where a large matrix product reaches 1320; 85 in fp32 (143).
+// 0.87 ms, 1016 TFLOP/s in bf16, where a large matrix product reaches 1320; 2 of up to 2048 rows, 16 heads, in fp32 77 (143).
 //
 // C layout of a 32x32 product: lane (h = lane / 32, c = lane % 32), register i: row 8 (i / 4) + 4 h + i % 4, column c.  With
 // rows = tokens, registers 8 s .. 8 s + 7 are the eight tokens {4 h + 0..3, 8 + 4 h + 0..3} of 16-token step s: the k
@@ -918,7 +918,8 @@ __device__ __forceinline__ void chunk_tile(const PageAttnArgs& a, const Split& s
 }
 
 // Workgroups of the short requests behind those of the long ones: they are bound by memory and fill what the last chunks
-// leave idle (12 requests, half of them single tokens, up to 512 rows and 16384 tokens: 558 us in two launches, 510 in one).
+// leave idle (12 requests, a third of them single tokens, up to 512 rows and 16384 tokens: 558 us in two launches and 510 in one as this
+// was built, 473 now).
 template <typename T, int DP, int DC>
 __global__ void __launch_bounds__(256, (ChunkTile<T, DP>::ROWB > 256 ? 1 : ChunkTile<T, DP>::ROWB > 128 ? 2 : 3))
     page_attn_chunk_kernel(const PageAttnArgs a, const Split sp, const Split step, const unsigned blocks) {
@@ -1075,12 +1076,13 @@ struct Plan {
 
 // Pieces of the key axis for a launch with `busy` workgroups per piece, by the longest request that the table can
 // describe: enough to fill the chip with 512 workgroups (two per CU) as long as a piece has 256 tokens, and up to `most`, which
-// the dispatcher can balance, as long as it has 2048.  Single tokens: 2 requests of up to 131072 tokens x 4 kv heads 77 us with
-// 64 pieces, 90 with 256; 64 x 8192 x 8 262 us with 4, 272 with 2.  Chunks, in the example above: 520 us with 2560, 534 with 2048,
-// 542 with 4096, 567 with 6144.  Below 768 tokens the join costs more than it saves (one token, 32 heads of 64 over 8 kv
+// the dispatcher can balance, as long as it has 2048.  Single tokens: 2 requests of up to 131072 tokens x 4 kv heads 76 us with
+// 64 pieces, 87 with 256; 64 x 8192 x 8 258 us with 4, 265 with 2.  Chunks, in the example above: 473 us with 2560, 483 with 2048,
+// 530 with 1280, 504 with 4096, 517 with 6144 (64 head dims: 269, 270, 319, 271, 276; in fp32, with 8 heads, with 24 requests or
+// under a window all alike).  Below 768 tokens the join costs more than it saves (one token, 32 heads of 64 over 8 kv
 // heads: 512 tokens 9.6 us cut, 7.8 whole; 1024 tokens 9.7 and 11.3).  Shorter requests have fewer pieces: chunks as many as
 // keep each within the longest's, so that no workgroup ends much later than the others; single tokens, which wait for memory
-// only, down to 512 tokens each (64 requests of 1 to 8192 tokens 307 us, 318 with the longest's, both with caches cold).
+// only, down to 512 tokens each (64 requests of 1 to 8192 tokens 238 us, 268 with the longest's, both with caches cold).
 void divide(const PageAttnArgs& a, Split& s, long long busy, int most, int log) {
   long long longest = (long long)a.width << a.shift;
   const long long seen = (long long)a.window + a.sinks + CHUNK_ROWS;
