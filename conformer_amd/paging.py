@@ -79,7 +79,10 @@ class KVPages:
                causal: bool = True, max_rows: int = 0) -> Tensor:
         """Attention of the step's rows [rows][heads][head_dim] over everything their requests hold in a layer, the rows'
         own keys included (write them first); see `ops.kv_page_attention`.  scale: 1 / sqrt(head_dim) if not given."""
+        step = self._open()
+        if q.shape[0] != step.slots.shape[0]:                 # the last requests' rows would sit at other positions
+            raise ValueError(f"KVPages: {q.shape[0]} rows of q in a step of {step.slots.shape[0]}")
         if scale is None:
             scale = q.shape[-1] ** -0.5
         return ops.kv_page_attention(q, self.k_pages[layer], self.v_pages[layer], self.block_table, self.kv_lens,
-                                     self._open().cu_rows, scale, window, sinks, causal, max_rows)
+                                     step.cu_rows, scale, window, sinks, causal, max_rows)

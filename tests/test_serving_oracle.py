@@ -285,3 +285,13 @@ def test_attention_workspace_follows_the_rows_of_the_step(batch, rows, max_rows,
     pair = 128 * 4 + 8
     need = N.lib().fcenc_page_attention_workspace_bytes(N.BF16, C.byref(pages), C.byref(r))
     assert need <= rows * heads * sum(pieces) * pair + 64
+
+
+@pytest.mark.parametrize("rows", [0, 4, 6])
+def test_cache_refuses_other_rows_than_the_step_has(rows):
+    """With fewer, the rows of the last request would be taken for its last ones."""
+    from conformer_amd.paging import Step
+    c = KVPages(layers=1, pages=4, kv_heads=2, head_dim=64, batch=2, max_tokens=100, page_size=32, device="cpu")
+    c.step = Step(torch.arange(5), torch.tensor([0, 2, 5], dtype=torch.int32), torch.tensor([True, True]))
+    with pytest.raises(ValueError, match="rows"):
+        c.attend(0, torch.zeros(rows, 4, 64))
